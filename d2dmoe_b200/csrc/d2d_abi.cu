@@ -108,6 +108,100 @@ int d2d_prenorm_init(const void* x, const void* gamma, const void* beta_opt, flo
                              out_init_opt, N, d, dtype, (cudaStream_t)stream);
 }
 
+static bool params_ok(int dtype, int param_dtype) {
+  return dtype_ok(dtype) && (param_dtype == D2D_F32 || param_dtype == dtype);
+}
+
+int d2d_layer_norm_workspace_bytes(int64_t N, int d, size_t* bytes) {
+  if (!bytes || N < 0 || d < 1) return D2D_ERR_BAD_ARG;
+  *bytes = align_up(norm_workspace_bytes(N, d), 256);
+  return D2D_OK;
+}
+
+int d2d_layer_norm(const void* x, int64_t x_stride, const void* gamma_opt, const void* beta_opt, float eps, int kind,
+                   float gamma_offset, void* y, float* mean_opt, float* rstd_opt, int64_t N, int d, int dtype,
+                   int param_dtype, d2d_stream_t stream) {
+  if (!x || !y || N < 0 || d < 1 || x_stride < 0 || !(eps >= 0.f) ||
+      (kind != D2D_NORM_LAYER && kind != D2D_NORM_RMS))
+    return D2D_ERR_BAD_ARG;
+  if (!params_ok(dtype, param_dtype) || d > D2D_NORM_MAX_D) return D2D_ERR_UNSUPPORTED;
+  if (N == 0) return D2D_OK;
+  return launch_norm_forward(x, x_stride, gamma_opt, beta_opt, eps, kind, gamma_offset, y, mean_opt, rstd_opt, N, d,
+                             dtype, param_dtype, (cudaStream_t)stream);
+}
+
+int d2d_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* gamma_opt,
+                            int kind, float gamma_offset, const float* mean, const float* rstd, void* dx_opt,
+                            void* dgamma_opt, void* dbeta_opt, int64_t N, int d, int dtype, int param_dtype, void* ws,
+                            size_t ws_bytes, d2d_stream_t stream) {
+  if (!dy || !x || !rstd || N < 0 || d < 1 || x_stride < 0 || dy_stride < 0 ||
+      (kind != D2D_NORM_LAYER && kind != D2D_NORM_RMS) || (kind == D2D_NORM_LAYER && !mean))
+    return D2D_ERR_BAD_ARG;
+  if (!params_ok(dtype, param_dtype) || d > D2D_NORM_MAX_D) return D2D_ERR_UNSUPPORTED;
+  if (!dx_opt && !dgamma_opt && !dbeta_opt) return D2D_OK;
+  if (N > 0 && (dgamma_opt || dbeta_opt)) {
+    if (!ws || !aligned(ws, 16)) return D2D_ERR_BAD_ARG;
+    if (ws_bytes < norm_workspace_bytes(N, d)) return D2D_ERR_WORKSPACE;
+  }
+  return launch_norm_backward(dy, dy_stride, x, x_stride, gamma_opt, kind, gamma_offset,
+                              kind == D2D_NORM_LAYER ? mean : nullptr, rstd, dx_opt, dgamma_opt, dbeta_opt, N, d,
+                              dtype, param_dtype, ws, (cudaStream_t)stream);
+}
+
+int d2d_route(const void* logits, const float* bias_opt, int scores, int k, int groups, int top_groups,
+              int renormalise, float scale, int32_t* experts, float* weights, uint32_t* mask_bits_opt,
+              void* routing_tensor_opt, int64_t N, int E, int dtype, d2d_stream_t stream) {
+  if (!logits || !experts || !weights || N < 0 || E < 1 || k < 1 || k > E || groups < 1 || E % groups != 0 ||
+      top_groups < 1 || top_groups > groups || k > E / groups * top_groups ||
+      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
+    return D2D_ERR_BAD_ARG;
+  if (!dtype_ok(dtype) || !route_supported(E, k, groups)) return D2D_ERR_UNSUPPORTED;
+  if (N == 0) return D2D_OK;
+  return launch_route(logits, bias_opt, k, scores == D2D_SCORES_SOFTMAX, renormalise != 0, scale, groups, top_groups,
+                      experts, weights, mask_bits_opt, routing_tensor_opt, N, E, dtype, (cudaStream_t)stream);
+}
+
+int d2d_route_backward(const void* logits, const int32_t* experts, const float* weights, const float* dweights,
+                       int scores, int renormalise, float scale, void* dlogits, int64_t N, int E, int k, int dtype,
+                       d2d_stream_t stream) {
+  if (!logits || !experts || !weights || !dweights || !dlogits || N < 0 || E < 1 || k < 1 || k > E ||
+      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
+    return D2D_ERR_BAD_ARG;
+  if (!dtype_ok(dtype) || !route_supported(E, k, 1)) return D2D_ERR_UNSUPPORTED;
+  if (N == 0) return D2D_OK;
+  return launch_route_backward(logits, experts, weights, dweights, scores == D2D_SCORES_SOFTMAX, renormalise != 0,
+                               scale, dlogits, N, E, k, dtype, (cudaStream_t)stream);
+}
+
+int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int dtype, size_t* bytes) {
+  if (!bytes || N < 0 || d < 1 || E < 1 || H < 1 || k < 1 || k > E) return D2D_ERR_BAD_ARG;
+  if (!dtype_ok(dtype)) return D2D_ERR_UNSUPPORTED;
+  *bytes = weighted_workspace_bytes(N, d, E, H, k, glu != 0, dtype);
+  return D2D_OK;
+}
+
+int d2d_experts_weighted(const void* x, const int32_t* experts, const float* weights, const void* w1,
+                         const void* b1_opt, const void* w_up_opt, const void* w2, const void* experts_packed_opt,
+                         const void* last_bias_opt, int add_residual, void* out, int64_t N, int d, int E, int H, int k,
+                         int act, int dtype, void* ws, size_t ws_bytes, int* dev_status, d2d_stream_t stream) {
+  if (!x || !experts || !weights || !w1 || !w2 || !out || N < 0 || d < 1 || E < 1 || H < 1 || k < 1 || k > E ||
+      (add_residual != 0 && add_residual != 1))
+    return D2D_ERR_BAD_ARG;
+  const size_t es = dtype == D2D_F32 ? 4 : 2;
+  if (!dtype_ok(dtype) || act < D2D_RELU || act > D2D_GELU_TANH) return D2D_ERR_UNSUPPORTED;
+  if (!aligned(x, es) || !aligned(out, es) || !aligned(experts, 4) || !aligned(weights, 4)) return D2D_ERR_BAD_ARG;
+  const bool glu = w_up_opt != nullptr;
+  const bool tiles = experts_packed_opt && aligned(experts_packed_opt, 1024) && aligned(x, 16) &&
+                     umma_experts_supported(d, E, H, glu, dtype);
+  if (!weighted_supported(N, d, E, H, k, glu, tiles)) return D2D_ERR_UNSUPPORTED;
+  if (N == 0) return D2D_OK;
+  if (!ws || !aligned(ws, 256)) return D2D_ERR_BAD_ARG;
+  if (ws_bytes < weighted_workspace_bytes(N, d, E, H, k, glu, dtype)) return D2D_ERR_WORKSPACE;
+  const WeightedCall c = {x,       w1,  b1_opt, w_up_opt, w2, tiles ? experts_packed_opt : nullptr, last_bias_opt,
+                          experts, weights, out, N, d, E, H, k, act, dtype, add_residual, dev_status};
+  return launch_weighted(c, ws, (cudaStream_t)stream);
+}
+
 int d2d_expand_mask(const uint32_t* mask_bits, void* routing_tensor, int64_t N, int E, int dtype,
                     d2d_stream_t stream) {
   if (!mask_bits || !routing_tensor || N < 0 || E < 1) return D2D_ERR_BAD_ARG;

@@ -216,6 +216,37 @@ int launch_init_out(const void* x, const void* last_bias, int add_residual, void
 int launch_prenorm_init(const void* x, const void* gamma, const void* beta, float eps, int kind,
                         float gamma_offset, const void* last_bias, void* xn, void* out, int64_t N,
                         int d, int dtype, cudaStream_t s);
+// row and parameter norms with statistics, any row length and stride (d2d_norm.cu)
+size_t norm_workspace_bytes(int64_t N, int d);
+int launch_norm_forward(const void* x, int64_t x_stride, const void* gamma, const void* beta, float eps,
+                        int kind, float offset, void* y, float* mean, float* rstd, int64_t N, int d,
+                        int dtype, int param_dtype, cudaStream_t s);
+int launch_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                         const void* gamma, int kind, float offset, const float* mean, const float* rstd,
+                         void* dx, void* dgamma, void* dbeta, int64_t N, int d, int dtype, int param_dtype,
+                         void* ws, cudaStream_t s);
+// token-choice routing and its gradient (d2d_route.cu)
+bool route_supported(int E, int k, int groups);
+int launch_route(const void* logits, const float* bias, int k, bool softmax, bool renormalise, float scale,
+                 int groups, int top_groups, int32_t* experts, float* weights, uint32_t* mask_bits, void* dense,
+                 int64_t N, int E, int dtype, cudaStream_t s);
+int launch_route_backward(const void* logits, const int32_t* experts, const float* weights,
+                          const float* dweights, bool softmax, bool renormalise, float scale, void* dlogits,
+                          int64_t N, int E, int k, int dtype, cudaStream_t s);
+// experts weighted by a routing (d2d_weighted.cu)
+struct WeightedCall {
+  const void *x, *w1, *b1, *w_up, *w2, *packed, *last_bias;      // packed: null where the shape has no such form
+  const int32_t* experts;      // [N, k], -1: none
+  const float* weights;        // [N, k]
+  void* out;
+  int64_t N;
+  int d, E, H, k, act, dtype, add_residual;
+  int* dev_status;
+};
+size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, int dtype);
+// tiles: the tensor-core kernel takes the shape
+bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, bool tiles);
+int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s);
 int launch_expand_mask(const uint32_t* mask_bits, void* rt, int64_t N, int E, int dtype,
                        cudaStream_t s);
 int launch_pack_mask(const void* rt, uint32_t* mask_bits, int64_t N, int E, int dtype,
@@ -239,6 +270,11 @@ int launch_router_fp32(const void* x, const void* wa, const void* wb, float mult
 int launch_experts_fp32(const void* x, const int32_t* token_idx, const int32_t* offsets,
                         const void* w1, const void* b1, const void* w2, void* out, int64_t N, int d,
                         int E, int H, int act, int* dev_status, cudaStream_t s, int kept);
+bool experts_simt_fits(int H, bool glu);      // the general-shape kernel's shared memory
+// Lists of pairs p = token k + slot: out row p = the expert's output for the token, stored (see d2d_weighted.cu)
+int launch_experts_simt_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,
+                              const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d,
+                              int E, int H, int k, int act, int dtype, int* dev_status, cudaStream_t s);
 // kept: experts that a token keeps, 0 where the rule leaves it open
 int launch_experts_simt(const void* x, const int32_t* token_idx, const int32_t* offsets,
                         const void* w1, const void* b1, const void* w_up, const void* w2,

@@ -51,13 +51,21 @@ inline Geo experts_geo(int d, int H, bool glu, long long n) {
 // 16 hidden columns as 8 packed bf16 pairs, with the upstream rounding points
 // (T(x W1), + b1, activation, x T(x W_up)) done in packed bf16 arithmetic: one
 // float->bf16x2 conversion per pair instead of one conversion per rounding point.
+// ONCE: in 32 bits instead, with one rounding at the end (the weighted form, which upstream has not).
 // NORM: nacc also collects the row's norm terms of the activation (before the gating
 // product), 1 = magnitudes, 2 = squares.
-template <int ACT, bool GLU, bool NORM>
+template <int ACT, bool GLU, bool NORM, bool ONCE = false>
 __device__ __forceinline__ void ep1_pairs(const uint32_t* v, const uint32_t* u, const uint32_t* bp,
                                           uint32_t* w, float& nacc, int nord) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
+    if (ONCE) {
+      float f0 = activate(__uint_as_float(v[2 * q]) + __uint_as_float(bp[q] << 16), ACT);
+      float f1 = activate(__uint_as_float(v[2 * q + 1]) + __uint_as_float(bp[q] & 0xffff0000u), ACT);
+      if (GLU) f0 *= __uint_as_float(u[2 * q]), f1 *= __uint_as_float(u[2 * q + 1]);
+      w[q] = pack_bf16x2(f0, f1);
+      continue;
+    }
     __nv_bfloat162 h =
         __floats2bfloat162_rn(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
     h = __hadd2_rn(h, *reinterpret_cast<const __nv_bfloat162*>(&bp[q]));

@@ -39,14 +39,15 @@ __device__ __forceinline__ void add_row_norms(const float* part, float* rown, in
 
 // TM_ rows per work item: 32, or 16 for small batches (more, lighter work items: with few
 // tokens the launch is one work item per SM and its duration is that item's).
-template <typename T, bool GLU, int TM_>
+// PAIRS: the lists hold pairs p = token * slots + slot; out row p is stored, nothing is rounded before it.
+template <typename T, bool GLU, int TM_, bool PAIRS>
 __global__ void __launch_bounds__(NT)
 experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_idx,
                     const int32_t* __restrict__ offsets, const T* __restrict__ w1,
                     const T* __restrict__ b1, const T* __restrict__ w_up,
                     const T* __restrict__ w2, T* __restrict__ out, int64_t N, int d, int E, int H,
                     int act, int* dev_status, T* __restrict__ norms, int norm_layer,
-                    int norm_ord) {
+                    int norm_ord, int slots) {
   extern __shared__ float sm[];
   constexpr int RG = TM_ / 16, CG = 8 / RG, CW = CB / CG, LC = CW / 4, LR = 32 / LC, RPT = 16 / LR;
   float* xs = sm;                              // [TM_][XP]
@@ -55,7 +56,9 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
   float* hs = wu + (GLU ? KC * WP : 0);        // [TM_][HP]
   const int HP = ((H + 3) & ~3) + 4;
   __shared__ int tstart[MAX_E + 1];
-  __shared__ int rows[TM_MAX];
+  __shared__ int rows[TM_MAX];                 // of out
+  __shared__ int tokens[PAIRS ? TM_MAX : 1];   // rows of x, where they are others
+  const int* const xrows = PAIRS ? tokens : rows;
   __shared__ float rown[TM_MAX];               // row sums of the norm by-product
   const int tid = threadIdx.x, lane = tid & 31, ty = tid >> 5;
   // Thread tile of both products: the 8 warps as RG (rows) x CG (columns), lanes LR x LC;
@@ -100,8 +103,9 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
     __syncthreads();
     if (tid < TM_) {
       int t = tid < nrows ? token_idx[r0 + tid] : -1;
-      if (tid < nrows && (t < 0 || t >= N)) { report(dev_status, D2D_ERR_INDEX_RANGE); t = -1; }
+      if (tid < nrows && (t < 0 || t >= (PAIRS ? N * slots : N))) { report(dev_status, D2D_ERR_INDEX_RANGE); t = -1; }
       rows[tid] = t;
+      if (PAIRS) tokens[tid] = t < 0 ? -1 : t / slots;
       rown[tid] = 0.f;
     }
     __syncthreads();
@@ -125,7 +129,7 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
       const int wk = tid >> 5, wc = (tid & 31) << 2;         // weight tile: k row (+8 per pass), column
       float4 px = z4, pw[4], pu[4];
       auto prefetch1 = [&](int kc) {
-        const int t = xr < TM_ ? rows[xr] : -1;
+        const int t = xr < TM_ ? xrows[xr] : -1;
         px = (t >= 0 && kc + xk < d) ? load4(x + (int64_t)t * d + kc + xk) : z4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -149,7 +153,7 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
         } else {
           for (int i = tid; i < TM_ * KC; i += NT) {
             const int r = i / KC, k = i % KC;
-            const int t = rows[r];
+            const int t = xrows[r];
             xs[r * XP + k] =
                 (t >= 0 && kc + k < d) ? DT<T>::to_f(x[(int64_t)t * d + kc + k]) : 0.f;
           }
@@ -209,6 +213,12 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
         for (int j = 0; j < 4; ++j) {
           const int c = hc + col0 + j;
           if (c < H) {
+            if (PAIRS) {
+              float h = b1 ? acc[i][j] + DT<T>::to_f(b1[(int64_t)e * H + c]) : acc[i][j];
+              h = activate(h, act);
+              hs[(row0 + LR * i) * HP + c] = GLU ? h * accu[i][j] : h;
+              continue;
+            }
             float h = DT<T>::round(acc[i][j]);
             if (b1) h = DT<T>::round(h + DT<T>::to_f(b1[(int64_t)e * H + c]));
             h = DT<T>::round(activate(h, act));
@@ -314,7 +324,11 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
         const int t = rows[row0 + LR * i];
         if (t < 0 || c0 >= d) continue;
         T* o = out + (int64_t)t * d + c0;
-        if (vec_ok) {
+        if (PAIRS) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c0 + j < d) o[j] = DT<T>::from_f(acc[i][j]);
+        } else if (vec_ok) {
           red_add_v4(o, DT<T>::round(acc[i][0]), DT<T>::round(acc[i][1]),
                      DT<T>::round(acc[i][2]), DT<T>::round(acc[i][3]));
         } else {
@@ -334,15 +348,19 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
   }
 }
 
-template <typename T, bool GLU, int TM_>
+size_t smem_bytes(int H, bool glu, int rows) {
+  const int HP = ((H + 3) & ~3) + 4;
+  return sizeof(float) * ((size_t)rows * XP + (size_t)KC * WP * (glu ? 2 : 1) + (size_t)rows * HP);
+}
+constexpr size_t SMEM_MOST = 200 * 1024;
+
+template <typename T, bool GLU, int TM_, bool PAIRS>
 int launch_tm(const void* x, const int32_t* token_idx, const int32_t* offsets, const void* w1,
               const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d, int E,
-              int H, int act, int* dev_status, cudaStream_t s, NormCapture nc) {
-  const int HP = ((H + 3) & ~3) + 4;
-  const size_t smem =
-      sizeof(float) * ((size_t)TM_ * XP + (size_t)KC * WP * (GLU ? 2 : 1) + (size_t)TM_ * HP);
-  if (smem > 200 * 1024) return D2D_ERR_UNSUPPORTED;
-  auto k = experts_simt_kernel<T, GLU, TM_>;
+              int H, int act, int* dev_status, cudaStream_t s, NormCapture nc, int slots) {
+  const size_t smem = smem_bytes(H, GLU, TM_);
+  if (smem > SMEM_MOST) return D2D_ERR_UNSUPPORTED;
+  auto k = experts_simt_kernel<T, GLU, TM_, PAIRS>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess)
     return D2D_ERR_LAUNCH;
@@ -350,7 +368,7 @@ int launch_tm(const void* x, const int32_t* token_idx, const int32_t* offsets, c
   const int grid = (int)(max_tiles < 148 * 4 ? (max_tiles > 0 ? max_tiles : 1) : 148 * 4);
   return launch_pdl(k, dim3((unsigned)grid), dim3(NT), smem, s, (const T*)x, token_idx, offsets,
                     (const T*)w1, (const T*)b1, (const T*)w_up, (const T*)w2, (T*)out, N, d, E, H,
-                    act, dev_status, (T*)nc.norms, nc.norms ? nc.layer : 0, nc.ord);
+                    act, dev_status, (T*)nc.norms, nc.norms ? nc.layer : 0, nc.ord, slots);
 }
 
 // 32-row work items.  (16-row items, instantiable through TM_, were measured on the 1576-token
@@ -360,8 +378,8 @@ template <typename T, bool GLU>
 int launch_t(const void* x, const int32_t* token_idx, const int32_t* offsets, const void* w1,
              const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d, int E,
              int H, int act, int* dev_status, cudaStream_t s, NormCapture nc) {
-  return launch_tm<T, GLU, 32>(x, token_idx, offsets, w1, b1, w_up, w2, out, N, d, E, H, act,
-                               dev_status, s, nc);
+  return launch_tm<T, GLU, 32, false>(x, token_idx, offsets, w1, b1, w_up, w2, out, N, d, E, H, act,
+                                      dev_status, s, nc, 1);
 }
 
 }  // namespace
@@ -386,6 +404,17 @@ int launch_experts_simt(const void* x, const int32_t* token_idx, const int32_t* 
                                      dev_status, s, nc)
               : launch_t<bf16, false>(x, token_idx, offsets, w1, b1, w_up, w2, out, N, d, E, H,
                                       act, dev_status, s, nc);
+}
+
+bool experts_simt_fits(int H, bool glu) { return smem_bytes(H, glu, 32) <= SMEM_MOST; }
+
+int launch_experts_simt_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,
+                              const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d,
+                              int E, int H, int k, int act, int dtype, int* dev_status, cudaStream_t s) {
+  if (E > MAX_E) return D2D_ERR_UNSUPPORTED;
+  const auto launch = dtype == D2D_F32 ? (w_up ? launch_tm<float, true, 32, true> : launch_tm<float, false, 32, true>)
+                                       : (w_up ? launch_tm<bf16, true, 32, true> : launch_tm<bf16, false, 32, true>);
+  return launch(x, pairs, offsets, w1, b1, w_up, w2, out, N, d, E, H, act, dev_status, s, NormCapture(), k);
 }
 
 }  // namespace d2d

@@ -77,6 +77,7 @@ struct Params {
   bool warm;                   // list and gather warps: a first pass without data, see role_list
   bf16* norms;                 // optional: [E, N] norms of each computed pair's activations
   int norm_layer, norm_ord;    // D2D_NORM_OF_INTERMEDIATE / D2D_NORM_OF_OUTPUT (0: none); 1 or 2
+  int slots;                   // lists of pairs: slots per token
 };
 
 struct Tile {
@@ -466,6 +467,8 @@ __device__ void role_list(const Params& p, Ctl* c, int lane, bool one_window) {
 // while its rows are copied, and so do the next tile's table words where that tile is known by then.  The
 // selection itself stands between two tiles' copies: a gated expert with two rows per 128-token tile makes it
 // search 64 of those for one of its own.)
+// PAIRS: the list holds pairs token * slots + slot; its rows of out are theirs alone and are stored.
+template <bool PAIRS>
 __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int lane) {
   volatile int* af = &c->abort_flag;
   const int j = lane & 7, row = w * 32 + lane;
@@ -497,7 +500,7 @@ __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int l
     }
     int tok = (int)x[0].x;
     if (tabled) tok = find_token(p, t, x, row, lane, live);
-    if (row < nrows && (tok < 0 || tok >= p.N)) {
+    if (row < nrows && (tok < 0 || tok >= (PAIRS ? p.N * p.slots : p.N))) {
       report(p.dev_status, D2D_ERR_INDEX_RANGE);
       tok = -1;
     }
@@ -515,7 +518,9 @@ __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int l
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int v = __shfl_sync(0xffffffffu, tok, i * 4 + (lane >> 3));
-      src[i] = p.x + (size_t)max(v < 0 ? v0 : v, 0) * p.d + j * 8;
+      uint32_t from = (uint32_t)max(v < 0 ? v0 : v, 0);
+      if (PAIRS) from /= (uint32_t)p.slots;
+      src[i] = p.x + (size_t)from * p.d + j * 8;
     }
     if (!live) {                         // the previous kernel's results from here on
       grid_dependency_wait();
@@ -548,7 +553,7 @@ __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int l
     }
     const uint32_t d = __ballot_sync(
         0xffffffffu, __popc(mask[0]) + __popc(mask[1]) + __popc(mask[2]) + __popc(mask[3]) == 1);
-    if (lane == 0) c->tile[q0.s].direct[w] = d;
+    if (lane == 0) c->tile[q0.s].direct[w] = PAIRS ? 0xffffffffu : d;
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(smem_u32(&c->rows_full[q0.s]));
@@ -704,7 +709,7 @@ __device__ void role_mma2(const Params& p, Ctl* c, uint32_t ring2, uint32_t tmem
 
 // Warps 0-3, thread = tile row = TMEM lane: accumulator 1 -> bias, activation (x
 // up-projection) -> bf16 hidden tile over the columns already read.
-template <int ACT, bool GLU, bool NORM>
+template <int ACT, bool GLU, bool NORM, bool ONCE>
 __device__ void role_ep1(const Params& p, Ctl* c, uint32_t tmem, int et) {
   volatile int* af = &c->abort_flag;
   const uint32_t lane_base = (uint32_t)(et & ~31) << 16;
@@ -734,7 +739,7 @@ __device__ void role_ep1(const Params& p, Ctl* c, uint32_t tmem, int et) {
       bb[0] = q0.x; bb[1] = q0.y; bb[2] = q0.z; bb[3] = q0.w;
       bb[4] = q1.x; bb[5] = q1.y; bb[6] = q1.z; bb[7] = q1.w;
       tmem_wait_ld();
-      ep1_pairs<ACT, GLU, NORM>(v, u, bb, w, nacc, nord);
+      ep1_pairs<ACT, GLU, NORM, ONCE>(v, u, bb, w, nacc, nord);
       tmem_st8(acc + (c0 >> 1), w);
     }
     tmem_wait_st();
@@ -750,14 +755,14 @@ __device__ void role_ep1(const Params& p, Ctl* c, uint32_t tmem, int et) {
   }
 }
 
-template <bool GLU, bool NORM>
+template <bool GLU, bool NORM, bool ONCE>
 __device__ __forceinline__ void role_ep1_act(const Params& p, Ctl* c, uint32_t tmem, int et) {
   switch (p.act) {         // one loop per activation: no branch inside
-    case D2D_RELU: role_ep1<D2D_RELU, GLU, NORM>(p, c, tmem, et); break;
-    case D2D_GELU: role_ep1<D2D_GELU, GLU, NORM>(p, c, tmem, et); break;
-    case D2D_TANH: role_ep1<D2D_TANH, GLU, NORM>(p, c, tmem, et); break;
-    case D2D_LEAKY_RELU: role_ep1<D2D_LEAKY_RELU, GLU, NORM>(p, c, tmem, et); break;
-    default: role_ep1<D2D_GELU_TANH, GLU, NORM>(p, c, tmem, et); break;
+    case D2D_RELU: role_ep1<D2D_RELU, GLU, NORM, ONCE>(p, c, tmem, et); break;
+    case D2D_GELU: role_ep1<D2D_GELU, GLU, NORM, ONCE>(p, c, tmem, et); break;
+    case D2D_TANH: role_ep1<D2D_TANH, GLU, NORM, ONCE>(p, c, tmem, et); break;
+    case D2D_LEAKY_RELU: role_ep1<D2D_LEAKY_RELU, GLU, NORM, ONCE>(p, c, tmem, et); break;
+    default: role_ep1<D2D_GELU_TANH, GLU, NORM, ONCE>(p, c, tmem, et); break;
   }
 }
 
@@ -921,8 +926,8 @@ __device__ void role_drain(const Params& p, Ctl* c, uint32_t tmem, int j, int q4
 // ---------------------------------------------------------------------------
 // kernel
 // ---------------------------------------------------------------------------
-// NORM: 0 none, D2D_NORM_OF_INTERMEDIATE, D2D_NORM_OF_OUTPUT
-template <bool GLU, int NORM>
+// NORM: 0 none, D2D_NORM_OF_INTERMEDIATE, D2D_NORM_OF_OUTPUT.  PAIRS: see role_gather
+template <bool GLU, int NORM, bool PAIRS = false>
 __global__ void __launch_bounds__(NTHREADS, 1) experts_tiles_kernel(const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -988,15 +993,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) experts_tiles_kernel(const Params
   }
 
   if (warp < WARP_DRAIN0) {
-    role_ep1_act<GLU, NORM == D2D_NORM_OF_INTERMEDIATE>(p, c, tmem, tid);
+    role_ep1_act<GLU, NORM == D2D_NORM_OF_INTERMEDIATE, PAIRS>(p, c, tmem, tid);
   } else if (warp < WARP_GATHER0) {
     const int w = warp - WARP_DRAIN0;
-    if (NORM != D2D_NORM_OF_OUTPUT && p.mask_bits)
+    if constexpr (PAIRS)
+      role_drain<GLU, false, true>(p, c, tmem, w >> 2, w & 3, lane);
+    else if (NORM != D2D_NORM_OF_OUTPUT && p.mask_bits)
       role_drain<GLU, false, true>(p, c, tmem, w >> 2, w & 3, lane);
     else
       role_drain<GLU, NORM == D2D_NORM_OF_OUTPUT, false>(p, c, tmem, w >> 2, w & 3, lane);
   } else if (warp < WARP_MMA1) {
-    role_gather(p, c, ring, warp - WARP_GATHER0, lane);
+    role_gather<PAIRS>(p, c, ring, warp - WARP_GATHER0, lane);
     cp_async_wait_all();
   } else if (warp == WARP_MMA1) {
     if (elect_one()) role_mma1<GLU>(p, c, ring, tmem);
@@ -1141,6 +1148,35 @@ int launch_experts_umma(const void* x, int32_t* token_idx, int32_t* offsets,
   const long long most = N * (long long)E * p.g.nc;
   const long long grid = most < sms ? most : sms;
   return launch_pdl(kernel, dim3((unsigned)grid), dim3(NTHREADS), smem, s, p);
+}
+
+int launch_experts_umma_pairs(const void* x, int32_t* pairs, int32_t* offsets, const void* packed, void* out,
+                              int64_t N, int d, int E, int H, int k, bool glu, int act, int* dev_status,
+                              cudaStream_t s) {
+  Params p = {};
+  p.x = (const bf16*)x;
+  p.N = N;
+  p.d = d;
+  p.E = E;
+  p.H = H;
+  p.act = act;
+  p.packed = (const uint8_t*)packed;
+  p.g = experts_geo(d, H, glu, N * k);     // (a token may want an expert twice)
+  p.token_idx = pairs;
+  p.offsets = offsets;
+  p.warm = true;
+  p.out = (bf16*)out;
+  p.dev_status = dev_status;
+  p.slots = k;
+  umma_debug_read(&p.wait_limit, &p.withhold);
+  const size_t smem =
+      1024 + (size_t)p.g.ns * p.g.stage + (size_t)p.g.ns2 * p.g.w2_piece + sizeof(Ctl) + 64;
+  const auto kernel = glu ? experts_tiles_kernel<true, 0, true> : experts_tiles_kernel<false, 0, true>;
+  int sms = 0;
+  const int rc = device_launch_facts((const void*)kernel, smem, &sms);
+  if (rc != D2D_OK) return rc;
+  const long long most = N * (long long)k * p.g.nc;      // see launch_experts_umma
+  return launch_pdl(kernel, dim3((unsigned)(most < sms ? most : sms)), dim3(NTHREADS), smem, s, p);
 }
 
 void umma_debug_read(uint32_t* wait_limit, int* withhold) {

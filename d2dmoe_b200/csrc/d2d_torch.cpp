@@ -526,7 +526,330 @@ PyObject* run_host(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- norm, routing and weighted experts -------------------------------------------
+// One call from Python per operator: arguments are checked, outputs and workspaces allocated on the current stream, the C
+// ABI entered.  Each returns its outputs, or the status code (int) of a refused call.
+
+// a tensor argument, which must be on the GPU (and on that of `like`); None: null
+const at::Tensor* given(PyObject* o, const char* name, const at::Tensor* like = nullptr) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor* t = tensor_of(o);
+  TORCH_CHECK_TYPE(t, name, " must be a tensor");
+  TORCH_CHECK(t->is_cuda(), "d2dmoe_b200 runs on CUDA tensors only (there is no CPU path)");
+  TORCH_CHECK_VALUE(!like || t->device() == like->device(), "tensors of one call live on different devices: ",
+                    like->device(), " and ", t->device(), " (", name, ")");
+  return t;
+}
+
+const at::Tensor& needed(PyObject* o, const char* name, const at::Tensor* like = nullptr) {
+  const at::Tensor* t = given(o, name, like);
+  TORCH_CHECK_TYPE(t, name, " must be a tensor");
+  return *t;
+}
+
+int dtype_of(const at::Tensor& t) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16,
+                   "d2dmoe_b200 supports float32 and bfloat16, got ", t.scalar_type());
+  return t.scalar_type() == at::kBFloat16 ? D2D_BF16 : D2D_F32;
+}
+
+void of_type(const at::Tensor& t, at::ScalarType s, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == s, name, " must be ", s, ", got ", t.scalar_type());
+}
+
+// [.., d] as rows: a matrix whose rows lie apart by any stride stays as it is, all else that is not contiguous is copied
+struct Rows {
+  at::Tensor t;
+  int64_t n, stride;
+};
+Rows rows_of(const at::Tensor& t) {
+  const int64_t d = t.size(-1);
+  if (t.dim() == 2 && (t.stride(1) == 1 || d == 1) && !t.is_contiguous()) return {t, t.size(0), t.stride(0)};
+  return {t.contiguous(), d > 0 ? t.numel() / d : 0, d};
+}
+
+// the stream, with the tensors' device current
+struct On {
+  c10::cuda::CUDAGuard guard;
+  d2d_stream_t stream;
+  explicit On(const at::Tensor& t)
+      : guard(t.device()), stream((d2d_stream_t)c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+void* data_or_null(const at::Tensor* t) { return t && t->defined() ? t->data_ptr() : nullptr; }
+
+PyObject* wrap(at::Tensor t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(t));
+}
+PyObject* wrap_all(std::initializer_list<at::Tensor> ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    PyObject* o = wrap(t);
+    if (!o) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+at::Tensor param_of(const at::Tensor* t, const char* name, int64_t d, at::ScalarType x, at::ScalarType* type) {
+  if (!t) return {};
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == d, name, " must have ", d, " values");
+  TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat || t->scalar_type() == x, name,
+                   " must be float32 or of x's dtype, got ", t->scalar_type());
+  TORCH_CHECK_TYPE(*type == at::ScalarType::Undefined || *type == t->scalar_type(),
+                   "weight and bias must be of one dtype");
+  *type = t->scalar_type();
+  return t->contiguous();
+}
+int param_code(at::ScalarType t, int x) {
+  return t == at::ScalarType::Undefined ? x : t == at::kFloat ? D2D_F32 : D2D_BF16;
+}
+
+// layer_norm(x, weight | None, bias | None, eps, kind, weight offset, statistics wanted) -> (y, mean | None, rstd | None)
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "layer_norm takes 7 arguments");
+  const at::Tensor& xt = needed(a[0], "x");
+  const int dt = dtype_of(xt);
+  TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) > 0, "x must have rows of one value or more");
+  const int64_t d = xt.size(-1);
+  at::ScalarType pt = at::ScalarType::Undefined;
+  const at::Tensor w = param_of(given(a[1], "weight", &xt), "weight", d, xt.scalar_type(), &pt);
+  const at::Tensor b = param_of(given(a[2], "bias", &xt), "bias", d, xt.scalar_type(), &pt);
+  const double eps = PyFloat_AsDouble(a[3]);
+  const int kind = (int)PyLong_AsLong(a[4]);
+  const double offset = PyFloat_AsDouble(a[5]);
+  const int stats = PyObject_IsTrue(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (d > D2D_NORM_MAX_D) return PyLong_FromLong(D2D_ERR_UNSUPPORTED);
+  On on(xt);
+  const Rows x = rows_of(xt);
+  at::Tensor y = at::detail::empty_cuda(xt.sizes(), xt.options()), mean, rstd;
+  if (stats) {
+    const auto f32 = xt.options().dtype(at::kFloat);
+    if (kind == D2D_NORM_LAYER) mean = at::detail::empty_cuda({x.n}, f32);
+    rstd = at::detail::empty_cuda({x.n}, f32);
+  }
+  const int rc = x.n == 0 ? D2D_OK
+                          : d2d_layer_norm(x.t.data_ptr(), x.stride, data_or_null(&w), data_or_null(&b), (float)eps,
+                                           kind, (float)offset, y.data_ptr(), (float*)data_or_null(&mean),
+                                           (float*)data_or_null(&rstd), x.n, (int)d, dt, param_code(pt, dt), on.stream);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({y, mean, rstd});
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_backward(dy, x, weight | None, mean | None, rstd, kind, weight offset, dx, dweight, dbias wanted)
+//   -> (dx, dweight, dbias), None where not wanted; without a weight the gradients are of x's dtype
+PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "layer_norm_backward takes 10 arguments");
+  const at::Tensor& xt = needed(a[1], "x");
+  const at::Tensor& gt = needed(a[0], "dy", &xt);
+  const int dt = dtype_of(xt);
+  of_type(gt, xt.scalar_type(), "dy");
+  TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) > 0, "x must have rows of one value or more");
+  TORCH_CHECK_VALUE(gt.sizes() == xt.sizes(), "dy must have the shape of x");
+  const int64_t d = xt.size(-1);
+  at::ScalarType pt = at::ScalarType::Undefined;
+  const at::Tensor w = param_of(given(a[2], "weight", &xt), "weight", d, xt.scalar_type(), &pt);
+  const at::Tensor* mean = given(a[3], "mean", &xt);
+  const at::Tensor& rstd = needed(a[4], "rstd", &xt);
+  const int kind = (int)PyLong_AsLong(a[5]);
+  const double offset = PyFloat_AsDouble(a[6]);
+  const int want[3] = {PyObject_IsTrue(a[7]), PyObject_IsTrue(a[8]), PyObject_IsTrue(a[9])};
+  if (PyErr_Occurred()) return nullptr;
+  if (d > D2D_NORM_MAX_D) return PyLong_FromLong(D2D_ERR_UNSUPPORTED);
+  On on(xt);
+  const Rows x = rows_of(xt), g = rows_of(gt);
+  for (const at::Tensor* t : {mean, &rstd})
+    if (t) {
+      of_type(*t, at::kFloat, "statistics");
+      TORCH_CHECK_VALUE(t->numel() == x.n && t->is_contiguous(), "mean and rstd must be contiguous, one value a row");
+    }
+  TORCH_CHECK_VALUE(kind != D2D_NORM_LAYER || mean, "mean is missing");
+  const auto po = xt.options().dtype(pt == at::ScalarType::Undefined ? xt.scalar_type() : pt);
+  at::Tensor dx, dw, db, ws;
+  if (want[0]) dx = at::detail::empty_cuda(xt.sizes(), xt.options());
+  if (want[1]) dw = at::detail::empty_cuda({d}, po);
+  if (want[2]) db = at::detail::empty_cuda({d}, po);
+  size_t bytes = 0;
+  if (want[1] || want[2]) {
+    const int rc = d2d_layer_norm_workspace_bytes(x.n, (int)d, &bytes);
+    if (rc != D2D_OK) return PyLong_FromLong(rc);
+    ws = at::detail::empty_cuda({(int64_t)std::max<size_t>(bytes, 16)}, xt.options().dtype(at::kByte));
+  }
+  // (tensors without rows have no address)
+  static float none;
+  const auto at_least = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : (void*)&none; };
+  const int rc = d2d_layer_norm_backward(
+      at_least(g.t), g.stride, at_least(x.t), x.stride, data_or_null(&w), kind, (float)offset,
+      mean ? (const float*)at_least(*mean) : nullptr, (const float*)at_least(rstd), x.n ? data_or_null(&dx) : nullptr,
+      data_or_null(&dw), data_or_null(&db), x.n, (int)d, dt, param_code(pt, dt), data_or_null(&ws), bytes, on.stream);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({dx, dw, db});
+  END_HANDLE_TH_ERRORS
+}
+
+// route(logits [N, E], k, scores, bias | None, groups, top_groups, renormalise, scale, mask bits | None, dense wanted)
+//   -> (weights, experts, routing tensor | None)
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "route takes 10 arguments");
+  const at::Tensor& lt = needed(a[0], "logits");
+  const int dt = dtype_of(lt);
+  TORCH_CHECK_VALUE(lt.dim() >= 1 && lt.size(-1) > 0, "logits must have one expert or more");
+  const int64_t E = lt.size(-1), N = lt.numel() / E;
+  const int64_t k = PyLong_AsLong(a[1]), scores = PyLong_AsLong(a[2]);
+  const at::Tensor* bt = given(a[3], "bias", &lt);
+  const int64_t groups = PyLong_AsLong(a[4]), top = PyLong_AsLong(a[5]);
+  const int renorm = PyObject_IsTrue(a[6]);
+  const double scale = PyFloat_AsDouble(a[7]);
+  const at::Tensor* mask = given(a[8], "mask bits", &lt);
+  const int dense = PyObject_IsTrue(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  if (E > (1 << 20) || k < 0 || k > E || groups < 0 || groups > E || top < 0 || top > E)
+    return PyLong_FromLong(E > (1 << 20) ? D2D_ERR_UNSUPPORTED : D2D_ERR_BAD_ARG);
+  On on(lt);
+  at::Tensor bias;
+  if (bt) {
+    of_type(*bt, at::kFloat, "bias");
+    TORCH_CHECK_VALUE(bt->dim() == 1 && bt->size(0) == E, "bias must have ", E, " values");
+    bias = bt->contiguous();
+  }
+  if (mask)
+    TORCH_CHECK_VALUE(mask->is_contiguous() && mask->element_size() == 4 && mask->numel() >= N * ((E + 31) / 32),
+                      "mask bits: room for [tokens, ceil(experts / 32)] words");
+  const at::Tensor logits = lt.contiguous();
+  c10::SmallVector<int64_t, 5> shape(lt.sizes().begin(), lt.sizes().end());
+  shape.back() = k;
+  at::Tensor w = at::detail::empty_cuda(shape, lt.options().dtype(at::kFloat));
+  at::Tensor e = at::detail::empty_cuda(shape, lt.options().dtype(at::kInt)), rt;
+  if (dense) rt = at::detail::empty_cuda(lt.sizes(), lt.options());
+  static int none;                       // (tensors without tokens have no address; arguments are checked all the same)
+  const int rc = d2d_route(N ? logits.data_ptr() : &none, (const float*)data_or_null(&bias), (int)scores, (int)k, (int)groups,
+                           (int)top, renorm, (float)scale, N ? (int32_t*)e.data_ptr() : &none,
+                           N ? (float*)w.data_ptr() : (float*)&none, (uint32_t*)data_or_null(mask), data_or_null(&rt), N,
+                           (int)E, dt, on.stream);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({w, e, rt});
+  END_HANDLE_TH_ERRORS
+}
+
+// route_backward(dweights, logits, experts, weights, scores, renormalise, scale) -> dlogits
+PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "route_backward takes 7 arguments");
+  const at::Tensor& lt = needed(a[1], "logits");
+  const at::Tensor& gt = needed(a[0], "dweights", &lt);
+  const at::Tensor& et = needed(a[2], "experts", &lt);
+  const at::Tensor& wt = needed(a[3], "weights", &lt);
+  const int dt = dtype_of(lt);
+  of_type(gt, at::kFloat, "dweights");
+  of_type(wt, at::kFloat, "weights");
+  of_type(et, at::kInt, "experts");
+  TORCH_CHECK_VALUE(lt.dim() >= 1 && lt.size(-1) > 0, "logits must have one expert or more");
+  const int64_t E = lt.size(-1), N = lt.numel() / E;
+  TORCH_CHECK_VALUE(et.dim() == lt.dim() && et.sizes().slice(0, et.dim() - 1) == lt.sizes().slice(0, lt.dim() - 1) &&
+                        wt.sizes() == et.sizes() && gt.sizes() == et.sizes(),
+                    "experts, weights and dweights must be [.., k] for logits [.., experts]");
+  const int64_t k = et.size(-1);
+  const int64_t scores = PyLong_AsLong(a[4]);
+  const int renorm = PyObject_IsTrue(a[5]);
+  const double scale = PyFloat_AsDouble(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (E > (1 << 20) || k > E) return PyLong_FromLong(k > E ? D2D_ERR_BAD_ARG : D2D_ERR_UNSUPPORTED);
+  On on(lt);
+  const at::Tensor logits = lt.contiguous(), e = et.contiguous(), w = wt.contiguous(), g = gt.contiguous();
+  at::Tensor out = at::detail::empty_cuda(lt.sizes(), lt.options());
+  static int none;
+  const auto at_least = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : (void*)&none; };
+  const int rc = d2d_route_backward(at_least(logits), (const int32_t*)at_least(e), (const float*)at_least(w),
+                                    (const float*)at_least(g), (int)scores, renorm, (float)scale, at_least(out), N,
+                                    (int)E, (int)k, dt, on.stream);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// experts_weighted(x [.., d], experts [.., k], weights [.., k], w1, b1 | None, w_up | None, w2, packed | None,
+//                  last bias | None, residual, act, status | None) -> out
+PyObject* experts_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 12, "experts_weighted takes 12 arguments");
+  const at::Tensor& xt = needed(a[0], "x");
+  const at::Tensor& et = needed(a[1], "experts", &xt);
+  const at::Tensor& wt = needed(a[2], "weights", &xt);
+  const at::Tensor& w1 = needed(a[3], "w1", &xt);
+  const at::Tensor* b1 = given(a[4], "b1", &xt);
+  const at::Tensor* up = given(a[5], "w_up", &xt);
+  const at::Tensor& w2 = needed(a[6], "w2", &xt);
+  const at::Tensor* packed = given(a[7], "packed weights", &xt);
+  const at::Tensor* bias = given(a[8], "last_bias", &xt);
+  const int residual = PyObject_IsTrue(a[9]);
+  const int act = (int)PyLong_AsLong(a[10]);
+  const at::Tensor* status = given(a[11], "status", &xt);
+  if (PyErr_Occurred()) return nullptr;
+  const int dt = dtype_of(xt);
+  of_type(et, at::kInt, "experts");
+  of_type(wt, at::kFloat, "weights");
+  TORCH_CHECK_VALUE(w1.dim() == 3 && w1.numel() > 0, "w1 must be [experts, d, expert width]");
+  const int64_t E = w1.size(0), d = w1.size(1), H = w1.size(2);
+  TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) == d, "x must be [.., ", d, "]");
+  const int64_t N = xt.numel() / d;
+  TORCH_CHECK_VALUE(et.dim() == xt.dim() && et.sizes().slice(0, et.dim() - 1) == xt.sizes().slice(0, xt.dim() - 1) &&
+                        wt.sizes() == et.sizes(),
+                    "experts and weights must be [.., k] for x [.., d]");
+  const int64_t k = et.size(-1);
+  const auto weight = [&](const at::Tensor& t, const char* name, at::IntArrayRef shape) {
+    of_type(t, xt.scalar_type(), name);
+    TORCH_CHECK_VALUE(t.sizes() == shape && t.is_contiguous(), name, " must be contiguous, of shape ", shape);
+  };
+  weight(w1, "w1", {E, d, H});
+  weight(w2, "w2", {E, H, d});
+  if (b1) weight(*b1, "b1", {E, H});
+  if (up) weight(*up, "w_up", {E, d, H});
+  if (bias) {
+    of_type(*bias, xt.scalar_type(), "last_bias");
+    TORCH_CHECK_VALUE(bias->numel() == d && bias->is_contiguous(), "last_bias must have ", d, " values");
+  }
+  if (packed) {
+    size_t most = 0;
+    const int rc = d2d_prepack_experts_bytes((int)d, (int)E, (int)H, up != nullptr, dt, &most);
+    TORCH_CHECK_VALUE(rc == D2D_OK && most > 0 && packed->is_contiguous() && packed->nbytes() >= most,
+                      "packed weights are not those of this shape");
+  }
+  if (k < 1 || k > E) return PyLong_FromLong(D2D_ERR_BAD_ARG);
+  On on(xt);
+  const at::Tensor x = xt.contiguous(), e = et.contiguous(), w = wt.contiguous();
+  at::Tensor out = at::detail::empty_cuda(xt.sizes(), xt.options()), ws;
+  size_t bytes = 0;
+  int rc = d2d_experts_weighted_workspace_bytes(N, (int)d, (int)E, (int)H, (int)k, up != nullptr, dt, &bytes);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  if (N > 0) {
+    ws = at::detail::empty_cuda({(int64_t)bytes}, xt.options().dtype(at::kByte));
+    rc = d2d_experts_weighted(x.data_ptr(), (const int32_t*)e.data_ptr(), (const float*)w.data_ptr(), w1.data_ptr(),
+                              data_or_null(b1), data_or_null(up), w2.data_ptr(), data_or_null(packed),
+                              data_or_null(bias), residual, out.data_ptr(), N, (int)d, (int)E, (int)H, (int)k, act, dt,
+                              ws.data_ptr(), bytes, (int*)data_or_null(status), on.stream);
+  }
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
+    {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
+    {"layer_norm_backward", (PyCFunction)(void (*)(void))layer_norm_backward, METH_FASTCALL, nullptr},
+    {"route", (PyCFunction)(void (*)(void))route, METH_FASTCALL, nullptr},
+    {"route_backward", (PyCFunction)(void (*)(void))route_backward, METH_FASTCALL, nullptr},
+    {"experts_weighted", (PyCFunction)(void (*)(void))experts_weighted, METH_FASTCALL, nullptr},
     {"mark", (PyCFunction)(void (*)(void))mark, METH_FASTCALL, nullptr},
     {"wait_mark", (PyCFunction)(void (*)(void))wait_mark, METH_FASTCALL, nullptr},
     {"make_pipe", (PyCFunction)(void (*)(void))make_pipe, METH_FASTCALL, nullptr},

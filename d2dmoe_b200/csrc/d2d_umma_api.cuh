@@ -23,6 +23,12 @@ int launch_experts_umma(const void* x, int32_t* token_idx, int32_t* offsets,
                         NormCapture nc = NormCapture(), DirectRows dr = DirectRows(),
                         const MaskTable* mt = nullptr);
 
+// Lists of pairs p = token k + slot (k: slots per token): out is [N k, d], row p is stored and is the expert's output for the
+// token; the hidden values are rounded once
+int launch_experts_umma_pairs(const void* x, int32_t* pairs, int32_t* offsets, const void* packed, void* out,
+                              int64_t N, int d, int E, int H, int k, bool glu, int act, int* dev_status,
+                              cudaStream_t s);
+
 bool umma_router_supported(int d, int R, int E, int dtype);
 size_t umma_router_packed_bytes(int d, int R, int E);
 int launch_prepack_router(const void* wa, const void* wb, void* packed, int d, int R, int E,

@@ -21,6 +21,7 @@ There is no CPU path: a forward on CPU tensors raises.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 
 import torch
 from torch import nn
@@ -156,6 +157,33 @@ class _PackedCache:
         return self._buf
 
 
+class _StatusWords(dict):
+    """Device status words of a module's weighted calls, one per device; copies start without any."""
+
+    def __missing__(self, device):
+        w = self[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        return w
+
+    def __deepcopy__(self, memo):
+        return _StatusWords()
+
+    def __reduce__(self):
+        return _StatusWords, ()
+
+
+@dataclass
+class Routing:
+    """How a layer in ``forward_mode = 'weighted'`` routes (see ``route_tokens``); the number of experts per token
+    is the layer's ``k``.  ``bias``: fp32 [experts] on the layer's device, or None."""
+
+    scores: str = "softmax"
+    bias: torch.Tensor | None = None
+    groups: int = 1
+    top_groups: int | None = None
+    renormalise: bool = True
+    scale: float = 1.0
+
+
 class ExpertIntermediateActivationExtractionStub(nn.Module):
     """Parameter-free hook point kept for attribute compatibility
     (architectures/moe/moe_layers.py:116-125); the fused kernel does not call it."""
@@ -227,6 +255,35 @@ class B200KernelExperts(ExpertsLayer):
     def invalidate_packed(self):
         """Drop the packed weight copy (needed only after writes through ``.data``)."""
         self._packed.invalidate()
+
+    # -- weighted form --------------------------------------------------------------------
+    @torch.no_grad()
+    def forward_weighted(self, x, experts, weights, last_bias=None, add_residual=False):
+        """``last_bias (+ x) + sum_j weights[.., j] * expert_{experts[.., j]}(x)`` for x [.., d] and what
+        ``route_tokens`` returns: experts [.., k] int32 (-1: no such slot), weights [.., k] fp32.  A token's sum is held in
+        fp32, in the order of its slots, and rounded once.  (Upstream multiplies every expert's output by its
+        routing entry, architectures/moe/moe_layers.py:91-101.)"""
+        self._check_mode()
+        if self._capture is not None:
+            raise NotImplementedError("activation norms are captured in the unweighted forms")
+        p = self.kernel_params()
+        return ops.experts_weighted(x, experts, weights, p["w1"], p["b1"], p["w2"], p["act"], w_up=p["w_up"],
+                                    packed=self.packed(), last_bias=last_bias, add_residual=add_residual,
+                                    status=self._status_words()[x.device])
+
+    def _status_words(self):
+        words = self.__dict__.get("_statuses")       # (not there in modules saved whole before it was)
+        if words is None:
+            words = self.__dict__["_statuses"] = _StatusWords()
+        return words
+
+    def check_status(self):
+        """Raise D2DError for what a kernel of an earlier ``forward_weighted`` reported (synchronises)."""
+        for w in self._status_words().values():
+            code = int(w.item())
+            if code:
+                w.zero_()
+                raise D2DError(code, "device status")
 
     # -- router-training labels as a by-product of the expert kernel ----------------------
     def capture_norms(self, layer, ord=2):
@@ -433,7 +490,8 @@ class MoeficationMoE(MoELayer):
 
     ``forward(x[B,S,d]) -> (out[B,S,d], {name: (routing_tensor[B,S,E],)})`` with
     ``forward_mode`` in {'all','topk','dynk','dynk_max'}, ``tau``/``k`` read at call
-    time.  In every mode the whole layer is one native call (router + rule -> bit mask ->
+    time; and 'weighted', which upstream has not: the router's output as logits of ``routing``
+    (a ``Routing``), ``k`` experts per token, their outputs weighted and summed; its routing tensor holds the weights.  In every mode the whole layer is one native call (router + rule -> bit mask ->
     token lists -> expert FFN with scatter-add); a router that is not the D2DMoE form runs as
     the module it is and hands over its scores.
     ``tau`` keeps the upstream meaning: expert e runs iff score_e >= max_e(score)*(1.0-tau).
@@ -464,6 +522,7 @@ class MoeficationMoE(MoELayer):
         self.router = None
         self.k = None
         self.tau = None
+        self.routing = Routing()
         self.add_residual_connection = add_residual_connection
         self._wsp = _WorkspaceCache()
         self._plan = _Plan()
@@ -471,7 +530,8 @@ class MoeficationMoE(MoELayer):
 
     def __setstate__(self, state):
         # modules saved whole before these attributes existed
-        super().__setstate__({"_plan": _Plan(), "_host": _HostBuffers(), **state})
+        super().__setstate__({"_plan": _Plan(), "_host": _HostBuffers(), "routing": Routing(),
+                              **state})
 
     # -- routing alone ------------------------------------------------------------
     def gate(self, x):
@@ -487,7 +547,23 @@ class MoeficationMoE(MoELayer):
             s2 = s.reshape(-1, s.size(-1)).contiguous()
             self._rule_mask(s2, wsp)
             return ops.expand_mask(wsp, s2.size(0), s2.size(1), s.dtype).view(s.shape)
+        if self.forward_mode == "weighted":
+            return self._route(x)[2]
         raise ValueError(f"Unsupported forward_mode: {self.forward_mode}")
+
+    def _route(self, x):
+        """(weights, experts, routing tensor) of the 'weighted' mode."""
+        r = self.routing
+        return ops.route(self.router(x), self.k, scores=r.scores, bias=r.bias, groups=r.groups,
+                         top_groups=r.top_groups, renormalise=r.renormalise, scale=r.scale, routing_tensor=True)
+
+    @torch.no_grad()
+    def _forward_weighted(self, x):
+        weights, experts, rt = self._route(x)
+        out = self.experts.forward_weighted(x, experts, weights,
+                                            last_bias=self.last_bias.view(-1) if self.bias else None,
+                                            add_residual=self.add_residual_connection)
+        return out, {self.name: (rt,)}
 
     def _rule_mask(self, s2, wsp):
         """Mask bits of the current routing rule from scores [N, E], on the device."""
@@ -578,6 +654,8 @@ class MoeficationMoE(MoELayer):
     def forward(self, x):
         ex = self._modules["experts"]
         rule = _RULES.get(self.forward_mode)
+        if rule is None and self.forward_mode == "weighted":
+            return self._forward_weighted(x)
         capture = getattr(ex, "_capture", None)
         if (rule is None or not x.is_cuda or ex._forward_mode not in _KERNEL_MODES
                 or (capture is not None and rule != ops.RULE_ALL)):

@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._capi import ACT, BF16, F32, check, lib
+from ._capi import ACT, BF16, F32, check, host, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
@@ -197,6 +197,75 @@ def prenorm_init(x2d, gamma, beta, eps: float, kind: int, xn, out_init=None, *, 
         check(lib.d2d_prenorm_init(_ptr(x2d), _ptr(gamma), _ptr(beta), float(eps), int(kind),
                                    float(gamma_offset), _ptr(last_bias), _ptr(xn), _ptr(out_init),
                                    N, d, _dt(x2d), st), "d2d_prenorm_init")
+
+
+_NORM_KIND = {"layer": NORM_LAYER, "rms": NORM_RMS}
+
+
+def norm_kind(kind: str) -> int:
+    if kind not in _NORM_KIND:
+        raise ValueError(f"unknown norm {kind!r}: 'layer' or 'rms'")
+    return _NORM_KIND[kind]
+
+
+def _refused(code, where):
+    """Raise for the status code of a refused native call; hand on what it returned otherwise."""
+    if type(code) is int:
+        raise _capi.D2DError(code, where)
+    return code
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, *, kind="layer", weight_offset=0.0,
+               statistics=True):
+    """``(y, mean, rstd)`` of rows x [.., d]: y = (x - mean) rstd (weight + weight_offset) + bias,
+    one value of mean and rstd per row in fp32 (RMS: no mean), or None without ``statistics``.
+    weight and bias: fp32 or x's dtype.  Rows of a matrix may lie apart by any stride.  Raises D2DError
+    UNSUPPORTED for rows of more than 16384 values."""
+    return _refused(host.layer_norm(x, weight, bias, eps, norm_kind(kind), weight_offset, statistics),
+                    "d2d_layer_norm")
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, *, kind="layer", weight_offset=0.0, bias=True,
+                        dx=True, dweight=True):
+    """``(dx, dweight, dbias)`` of ``layer_norm`` from its statistics; ``bias``, ``dx``, ``dweight``: which of
+    them are wanted (None otherwise).  The parameters' gradients are of the weight's dtype (x's without one)."""
+    return _refused(host.layer_norm_backward(dy, x, weight, mean, rstd, norm_kind(kind), weight_offset, dx,
+                                             dweight, bias), "d2d_layer_norm_backward")
+
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def score_kind(scores: str) -> int:
+    if scores not in SCORES:
+        raise ValueError(f"unknown scores {scores!r}: 'softmax' or 'sigmoid'")
+    return SCORES[scores]
+
+
+def route(logits, k, *, scores="softmax", bias=None, groups=1, top_groups=None, renormalise=True,
+          scale=1.0, wsp: Workspace | None = None, routing_tensor=False):
+    """Token-choice routing of logits [.., E] -> ``(weights [.., k] fp32, experts [.., k] int32, routing tensor
+    [.., E] in the logits' dtype or None)``; see ``d2d_route`` in include/d2dmoe.h for the rules.  ``wsp``: its
+    mask bits are written too, for ``compact``."""
+    if wsp is not None and logits.size(-1) != wsp.E:
+        raise ValueError(f"the workspace is for {wsp.E} experts, the logits have {logits.size(-1)}")
+    return _refused(host.route(logits, k, score_kind(scores), bias, groups,
+                               groups if top_groups is None else top_groups, renormalise, scale,
+                               None if wsp is None else wsp.mask_bits, routing_tensor), "d2d_route")
+
+
+def route_backward(dweights, logits, experts, weights, *, scores="softmax", renormalise=True, scale=1.0):
+    """Gradient of ``route``'s weights with respect to the logits, the choice held fixed."""
+    return _refused(host.route_backward(dweights, logits, experts, weights, score_kind(scores), renormalise,
+                                        scale), "d2d_route_backward")
+
+
+def experts_weighted(x, experts, weights, w1, b1, w2, act: str, *, w_up=None, packed=None, last_bias=None,
+                     add_residual=False, status=None):
+    """``last_bias (+ x) + sum_j weights[.., j] FFN_{experts[.., j]}(x)`` for x [.., d], experts [.., k] int32 (-1: no
+    such slot) and weights [.., k] fp32.  ``status`` [1] int32 receives D2D_ERR_INDEX_RANGE for other experts."""
+    return _refused(host.experts_weighted(x, experts, weights, w1, b1, w_up, w2, packed, last_bias,
+                                          add_residual, ACT[act], status), "d2d_experts_weighted")
 
 
 def compact(wsp: Workspace, N: int, E: int):

@@ -219,6 +219,73 @@ int d2d_prenorm_init(const void* x, const void* gamma, const void* beta_opt, flo
                      float gamma_offset, const void* last_bias_opt, void* xn, void* out_init_opt,
                      int64_t N, int d, int dtype, d2d_stream_t stream);
 
+/* The normalisation alone, for rows of any length up to D2D_NORM_MAX_D, with what its backward pass needs.
+ * y[t,:] = T(xh (gamma + gamma_offset) + beta), xh = (x[t,:] - mean) rstd, kinds as above (RMS: mean = 0);
+ * gamma_opt NULL: xh alone (gamma_offset is then not used), beta_opt NULL: nothing is added.
+ * x_stride: elements from one row of x to the next (>= 0; a row's elements lie together); y is [N, d].
+ * param_dtype: of gamma, beta and their gradients, D2D_F32 or dtype.  mean_opt, rstd_opt [N] fp32 receive the
+ * statistics.  fp32 statistics, one rounding to T.  Replaces torch's LayerNorm and the RMSNorm modules in front of
+ * the layer (architectures/moe/moe_models.py:69-76, :91-100, :148-156) where they are trained. */
+#define D2D_NORM_MAX_D 16384
+int d2d_layer_norm(const void* x, int64_t x_stride, const void* gamma_opt, const void* beta_opt, float eps, int kind,
+                   float gamma_offset, void* y, float* mean_opt, float* rstd_opt, int64_t N, int d, int dtype,
+                   int param_dtype, d2d_stream_t stream);
+
+/* Its backward pass: with g = dy (gamma + gamma_offset)
+ *   dx     = T(rstd (g - mean_d(g) - xh mean_d(g xh)))       (RMS: without mean_d(g); mean may be NULL)
+ *   dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy, in param_dtype
+ * from x and the forward pass's mean and rstd.  Each of the three outputs may be NULL.  The column sums are held in
+ * fp32 and taken in a fixed order: the same call gives the same bits.  N = 0 sets dgamma and dbeta to zero.
+ * ws: d2d_layer_norm_workspace_bytes(N, d), needed where dgamma or dbeta is. */
+int d2d_layer_norm_workspace_bytes(int64_t N, int d, size_t* bytes /* host */);
+int d2d_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* gamma_opt,
+                            int kind, float gamma_offset, const float* mean, const float* rstd, void* dx_opt,
+                            void* dgamma_opt, void* dbeta_opt, int64_t N, int d, int dtype, int param_dtype, void* ws,
+                            size_t ws_bytes, d2d_stream_t stream);
+
+/* Token-choice routing with weights, on the logits of any router:
+ *   s = softmax(logits) or sigmoid(logits);  c = s + bias_opt (fp32 [E]; without one the order of the logits)
+ *   groups > 1: the E experts are cut into `groups` equal parts, each of which counts as the sum of its two best c
+ *   (s without a bias); only experts of the top_groups best parts can be chosen
+ *   experts[t, 0..k-1] (i32) = the k best c of token t, the best first, ties to the lowest index
+ *   weights[t, j] (fp32) = scale s, or scale s / (sum of the chosen s) with renormalise
+ * The choice is made as 64-bit arithmetic makes it, whatever T is.  A logit of -inf (or a bias of -inf) takes an expert
+ * out of the choice; slots for which none is left have expert -1 and weight 0.  A token with a NaN or +inf among its
+ * logits or biases has experts -1 and weights NaN.  Optional outputs: mask_bits (what d2d_compact reads) and the
+ * routing tensor [N, E] in T with the weights in place of ones.
+ * 1 <= k <= min(32, E / groups * top_groups), E <= 1024, groups <= 32 divides E, scale > 0.
+ * (Upstream's 'topk' gate, architectures/moe/moefication.py:59-63, keeps 0/1 decisions of raw scores.) */
+#define D2D_SCORES_SOFTMAX 0
+#define D2D_SCORES_SIGMOID 1
+int d2d_route(const void* logits, const float* bias_opt, int scores, int k, int groups, int top_groups,
+              int renormalise, float scale, int32_t* experts, float* weights, uint32_t* mask_bits_opt,
+              void* routing_tensor_opt, int64_t N, int E, int dtype, d2d_stream_t stream);
+
+/* Gradient of d2d_route's weights with respect to the logits, the choice held fixed (it has none, nor has the bias):
+ * dlogits [N, E] in T from dweights [N, k] fp32 and what d2d_route returned.  Slots with an expert outside 0..E-1
+ * add nothing; tokens without any chosen expert get zeros. */
+int d2d_route_backward(const void* logits, const int32_t* experts, const float* weights, const float* dweights,
+                       int scores, int renormalise, float scale, void* dlogits, int64_t N, int E, int k, int dtype,
+                       d2d_stream_t stream);
+
+/* Experts weighted by a routing:
+ *   out[t,:] = T(last_bias_opt (+ x[t,:]) + sum_j weights[t,j] y[t,j,:]),
+ *   y[t,j,:] = act(x[t,:] W1[e] + b1[e]) (* x[t,:] W_up[e]) W2[e],  e = experts[t,j]
+ * for experts [N, k] (i32; -1: no such slot; the same expert may stand in several) and weights [N, k] (fp32).  A
+ * token's sum is held in fp32, taken in the order of its slots and rounded once.  The hidden values are
+ * rounded once (bf16 tensor-core path) or not at all, y to T, except in calls of few pairs, where nothing is
+ * rounded before the end.  The same call gives the same bits.  An expert outside -1..E-1 is skipped and reported
+ * (D2D_ERR_INDEX_RANGE in *dev_status).  k <= min(32, E), E <= 256, N k < 2^31 - 1.  experts_packed_opt as for
+ * d2d_experts_ffn; shapes and buffers that the tensor-core kernels do not take go to the general-shape ones.
+ * ws: d2d_experts_weighted_workspace_bytes, 256-byte aligned.  (Upstream's dense form multiplies every
+ * expert's output by its routing entry: architectures/moe/moe_layers.py:91-101.) */
+int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int dtype,
+                                         size_t* bytes /* host */);
+int d2d_experts_weighted(const void* x, const int32_t* experts, const float* weights, const void* w1,
+                         const void* b1_opt, const void* w_up_opt, const void* w2, const void* experts_packed_opt,
+                         const void* last_bias_opt, int add_residual, void* out, int64_t N, int d, int E, int H, int k,
+                         int act, int dtype, void* ws, size_t ws_bytes, int* dev_status, d2d_stream_t stream);
+
 /* add_residual values of d2d_moe_forward: 0 = out starts as last_bias, 1 = as last_bias + x
  * (MoeficationMoE.add_residual_connection, architectures/moe/moefication.py:98-99),
  * D2D_OUT_PREINITIALISED = out already holds its initial value (d2d_prenorm_init wrote it);
