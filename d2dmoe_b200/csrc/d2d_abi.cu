@@ -155,10 +155,15 @@ int d2d_route(const void* logits, const float* bias_opt, int scores, int k, int 
       top_groups < 1 || top_groups > groups || k > E / groups * top_groups ||
       (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
     return D2D_ERR_BAD_ARG;
-  if (!dtype_ok(dtype) || !route_supported(E, k, groups)) return D2D_ERR_UNSUPPORTED;
+  if (!dtype_ok(dtype) || E > ROUTE_MAX_E || k > ROUTE_MAX_K || groups > ROUTE_MAX_GROUPS)
+    return D2D_ERR_UNSUPPORTED;
   if (N == 0) return D2D_OK;
-  return launch_route(logits, bias_opt, k, scores == D2D_SCORES_SOFTMAX, renormalise != 0, scale, groups, top_groups,
-                      experts, weights, mask_bits_opt, routing_tensor_opt, N, E, dtype, (cudaStream_t)stream);
+  int sms = 0;
+  const int rc = device_launch_facts(nullptr, 0, &sms);
+  if (rc != D2D_OK) return rc;
+  const RouteCall c = {logits, bias_opt, experts, weights, mask_bits_opt, routing_tensor_opt, N, E, k, groups, top_groups,
+                       scores == D2D_SCORES_SOFTMAX, renormalise != 0, scale};
+  return (dtype == D2D_F32 ? launch_route_fp32 : launch_route_bf16)(c, sms, (cudaStream_t)stream);
 }
 
 int d2d_route_backward(const void* logits, const int32_t* experts, const float* weights, const float* dweights,
@@ -167,10 +172,15 @@ int d2d_route_backward(const void* logits, const int32_t* experts, const float* 
   if (!logits || !experts || !weights || !dweights || !dlogits || N < 0 || E < 1 || k < 1 || k > E ||
       (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
     return D2D_ERR_BAD_ARG;
-  if (!dtype_ok(dtype) || !route_supported(E, k, 1)) return D2D_ERR_UNSUPPORTED;
+  if (!dtype_ok(dtype) || E > ROUTE_MAX_E || k > ROUTE_MAX_K) return D2D_ERR_UNSUPPORTED;
   if (N == 0) return D2D_OK;
-  return launch_route_backward(logits, experts, weights, dweights, scores == D2D_SCORES_SOFTMAX, renormalise != 0,
-                               scale, dlogits, N, E, k, dtype, (cudaStream_t)stream);
+  int sms = 0;
+  const int rc = device_launch_facts(nullptr, 0, &sms);
+  if (rc != D2D_OK) return rc;
+  const RouteCall c = {logits, nullptr, const_cast<int32_t*>(experts), const_cast<float*>(weights), nullptr, nullptr, N, E,
+                       k, 1, 1, scores == D2D_SCORES_SOFTMAX, renormalise != 0, scale};
+  return (dtype == D2D_F32 ? launch_route_backward_fp32 : launch_route_backward_bf16)(c, dweights, dlogits, sms,
+                                                                                       (cudaStream_t)stream);
 }
 
 int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int dtype, size_t* bytes) {

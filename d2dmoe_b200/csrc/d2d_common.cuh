@@ -225,14 +225,24 @@ int launch_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64
                          const void* gamma, int kind, float offset, const float* mean, const float* rstd,
                          void* dx, void* dgamma, void* dbeta, int64_t N, int d, int dtype, int param_dtype,
                          void* ws, cudaStream_t s);
-// token-choice routing and its gradient (d2d_route.cu)
-bool route_supported(int E, int k, int groups);
-int launch_route(const void* logits, const float* bias, int k, bool softmax, bool renormalise, float scale,
-                 int groups, int top_groups, int32_t* experts, float* weights, uint32_t* mask_bits, void* dense,
-                 int64_t N, int E, int dtype, cudaStream_t s);
-int launch_route_backward(const void* logits, const int32_t* experts, const float* weights,
-                          const float* dweights, bool softmax, bool renormalise, float scale, void* dlogits,
-                          int64_t N, int E, int k, int dtype, cudaStream_t s);
+// token-choice routing and its gradient (d2d_route.cuh)
+struct RouteCall {
+  const void* logits;
+  const float* bias;           // optional
+  int32_t* experts;
+  float* weights;
+  uint32_t* mask_bits;         // optional
+  void* dense;                 // optional
+  int64_t N;
+  int E, k, groups, top_groups;
+  bool softmax, renormalise;
+  float scale;
+};
+constexpr int ROUTE_MAX_E = 1024, ROUTE_MAX_K = 32, ROUTE_MAX_GROUPS = 32;
+int launch_route_bf16(const RouteCall& c, int sms, cudaStream_t s);
+int launch_route_fp32(const RouteCall& c, int sms, cudaStream_t s);
+int launch_route_backward_bf16(const RouteCall& c, const float* dweights, void* dlogits, int sms, cudaStream_t s);
+int launch_route_backward_fp32(const RouteCall& c, const float* dweights, void* dlogits, int sms, cudaStream_t s);
 // experts weighted by a routing (d2d_weighted.cu)
 struct WeightedCall {
   const void *x, *w1, *b1, *w_up, *w2, *packed, *last_bias;      // packed: null where the shape has no such form

@@ -51,12 +51,15 @@ class _Route(torch.autograd.Function):
         weights, experts, _ = ops.route(logits, k, bias=bias, groups=groups, top_groups=top_groups, **how)
         ctx.save_for_backward(logits, experts, weights)
         ctx.how = how
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(experts)
         return weights, experts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dweights, _):
+        if dweights is None:
+            return (None,) * 6
         logits, experts, weights = ctx.saved_tensors
         return ops.route_backward(dweights, logits, experts, weights, **ctx.how), None, None, None, None, None
 
