@@ -52,7 +52,7 @@ SIGNATURES = {
                                      _i, _p, _sz, _p]),
     "d2d_route": (_i, [_p, _p, _i, _i, _i, _i, _i, _f, _p, _p, _p, _p, _i64, _i, _i, _p]),
     "d2d_route_backward": (_i, [_p, _p, _p, _p, _i, _i, _f, _p, _i64, _i, _i, _i, _p]),
-    "d2d_experts_weighted_workspace_bytes": (_i, [_i64, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "d2d_experts_weighted_workspace_bytes": (_i, [_i64, _i, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
     "d2d_experts_weighted": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _i,
                                   _i, _p, _sz, _p, _p]),
     "d2d_prepack_experts_bytes": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),

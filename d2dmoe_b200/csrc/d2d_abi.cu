@@ -183,10 +183,12 @@ int d2d_route_backward(const void* logits, const int32_t* experts, const float* 
                                                                                        (cudaStream_t)stream);
 }
 
-int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int dtype, size_t* bytes) {
+int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int packed, int dtype,
+                                         size_t* bytes) {
   if (!bytes || N < 0 || d < 1 || E < 1 || H < 1 || k < 1 || k > E) return D2D_ERR_BAD_ARG;
   if (!dtype_ok(dtype)) return D2D_ERR_UNSUPPORTED;
-  *bytes = weighted_workspace_bytes(N, d, E, H, k, glu != 0, dtype);
+  *bytes = weighted_workspace_bytes(N, d, E, H, k, glu != 0,
+                                    packed && umma_experts_supported(d, E, H, glu != 0, dtype));
   return D2D_OK;
 }
 
@@ -197,16 +199,16 @@ int d2d_experts_weighted(const void* x, const int32_t* experts, const float* wei
   if (!x || !experts || !weights || !w1 || !w2 || !out || N < 0 || d < 1 || E < 1 || H < 1 || k < 1 || k > E ||
       (add_residual != 0 && add_residual != 1))
     return D2D_ERR_BAD_ARG;
-  const size_t es = dtype == D2D_F32 ? 4 : 2;
   if (!dtype_ok(dtype) || act < D2D_RELU || act > D2D_GELU_TANH) return D2D_ERR_UNSUPPORTED;
-  if (!aligned(x, es) || !aligned(out, es) || !aligned(experts, 4) || !aligned(weights, 4)) return D2D_ERR_BAD_ARG;
   const bool glu = w_up_opt != nullptr;
-  const bool tiles = experts_packed_opt && aligned(experts_packed_opt, 1024) && aligned(x, 16) &&
-                     umma_experts_supported(d, E, H, glu, dtype);
+  const bool tiles = experts_packed_opt && umma_experts_supported(d, E, H, glu, dtype);
+  if (!aligned(x, 16) || !aligned(out, 16) || !aligned(experts, 4) || !aligned(weights, 4) ||
+      (tiles && (!aligned(experts_packed_opt, 1024) || !aligned(last_bias_opt, 16))))
+    return D2D_ERR_BAD_ARG;
   if (!weighted_supported(N, d, E, H, k, glu, tiles)) return D2D_ERR_UNSUPPORTED;
   if (N == 0) return D2D_OK;
   if (!ws || !aligned(ws, 256)) return D2D_ERR_BAD_ARG;
-  if (ws_bytes < weighted_workspace_bytes(N, d, E, H, k, glu, dtype)) return D2D_ERR_WORKSPACE;
+  if (ws_bytes < weighted_workspace_bytes(N, d, E, H, k, glu, tiles)) return D2D_ERR_WORKSPACE;
   const WeightedCall c = {x,       w1,  b1_opt, w_up_opt, w2, tiles ? experts_packed_opt : nullptr, last_bias_opt,
                           experts, weights, out, N, d, E, H, k, act, dtype, add_residual, dev_status};
   return launch_weighted(c, ws, (cudaStream_t)stream);

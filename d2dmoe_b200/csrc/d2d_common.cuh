@@ -49,6 +49,13 @@ __device__ __forceinline__ void grid_dependency_wait() {
 __device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// A pointer to what earlier kernels have written, behind the wait.  Loads that the compiler takes to be of constant
+// memory (__ldg, const __restrict__) do not heed the wait's clobber: without this it may move them above it.
+template <typename... Pointer>
+__device__ __forceinline__ void fresh(Pointer&... p) {
+  const int in_turn[] = {([](auto& q) { asm volatile("" : "+l"(q)); }(p), 0)...};
+  (void)in_turn;
+}
 // cluster > 0: in clusters of that many CTAs.
 template <typename... KArgs, typename... Args>
 inline int launch_pdl_cluster(int cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block,
@@ -253,7 +260,7 @@ struct WeightedCall {
   int d, E, H, k, act, dtype, add_residual;
   int* dev_status;
 };
-size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, int dtype);
+size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, bool tiles);
 // tiles: the tensor-core kernel takes the shape
 bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, bool tiles);
 int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s);
@@ -281,7 +288,7 @@ int launch_experts_fp32(const void* x, const int32_t* token_idx, const int32_t* 
                         const void* w1, const void* b1, const void* w2, void* out, int64_t N, int d,
                         int E, int H, int act, int* dev_status, cudaStream_t s, int kept);
 bool experts_simt_fits(int H, bool glu);      // the general-shape kernel's shared memory
-// Lists of pairs p = token k + slot: out row p = the expert's output for the token, stored (see d2d_weighted.cu)
+// Lists of pairs p = token k + slot: out row p [d] fp32 = the expert's output for the token (see d2d_weighted.cu)
 int launch_experts_simt_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,
                               const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d,
                               int E, int H, int k, int act, int dtype, int* dev_status, cudaStream_t s);

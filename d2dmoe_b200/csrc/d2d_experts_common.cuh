@@ -118,6 +118,59 @@ __device__ __forceinline__ void add_row(void* p, int t, uint4 v) {
       : "memory");
 }
 
+// Eight floats in 16 bytes: 15-bit integers in units of a common power of two, 2^-13 of the one above the largest.  A bf16 row
+// would be as large and 2^-9 off at every element; this is 2^-14 off of the largest of eight.  The exponent (that of the
+// largest, as floats have it) lies in the lowest bits of the eight halves.  Exponent 255, where one is not
+// finite: the halves are bf16 without their lowest bit.
+__device__ __forceinline__ uint4 encode8(const float (&f)[8]) {
+  float m = fabsf(f[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(f[i])));
+  uint32_t ex = __float_as_uint(m) >> 23;
+  uint32_t w[4];
+  if (ex == 255u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]) & 0xfffefffeu;
+  } else {
+    ex = max(ex, 13u);
+    const float s = __uint_as_float((266u - ex) << 23);      // 2^(139 - ex): |f s| < 2^13
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __float_as_uint(fmaf(f[2 * i], s, 12582912.f)),
+                     b = __float_as_uint(fmaf(f[2 * i + 1], s, 12582912.f));     // 1.5 2^23: the integer is below
+      w[i] = (__byte_perm(a, b, 0x5410) << 1) & 0xfffefffeu;
+    }
+  }
+  const uint32_t z = ex | ex << 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] |= (z >> (2 * i)) & 0x00010001u;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// sum += wt * the eight
+__device__ __forceinline__ void add_decoded8(uint4 v, float wt, float (&sum)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t ex = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = w[i] & 0x00010001u;
+    ex |= ((t | t >> 15) & 3u) << (2 * i);
+  }
+  if (ex == 255u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[2 * i] = fmaf(wt, __uint_as_float(w[i] << 16 & 0xfffe0000u), sum[2 * i]);
+      sum[2 * i + 1] = fmaf(wt, __uint_as_float(w[i] & 0xfffe0000u), sum[2 * i + 1]);
+    }
+    return;
+  }
+  const float s = __uint_as_float((ex - 12u) << 23);         // 2^(ex - 139)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[2 * i] = fmaf(wt, (float)((int32_t)(w[i] << 16) >> 17) * s, sum[2 * i]);
+    sum[2 * i + 1] = fmaf(wt, (float)((int32_t)w[i] >> 17) * s, sum[2 * i + 1]);
+  }
+}
+
 }  // namespace umma
 
 // Short calls (d2d_experts_short.cu)

@@ -39,7 +39,7 @@ __device__ __forceinline__ void add_row_norms(const float* part, float* rown, in
 
 // TM_ rows per work item: 32, or 16 for small batches (more, lighter work items: with few
 // tokens the launch is one work item per SM and its duration is that item's).
-// PAIRS: the lists hold pairs p = token * slots + slot; out row p is stored, nothing is rounded before it.
+// PAIRS: the lists hold pairs p = token * slots + slot; out row p is stored, in fp32, and nothing is rounded.
 template <typename T, bool GLU, int TM_, bool PAIRS>
 __global__ void __launch_bounds__(NT)
 experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_idx,
@@ -70,6 +70,7 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
   const int row0 = 16 * rg + lr, col0 = CW * cg + 4 * lc;
   grid_launch_dependents();
   grid_dependency_wait();      // token lists and offsets come from the previous kernel
+  if (PAIRS) fresh(x, token_idx, offsets, w1, b1, w_up, w2);
 
   if (tid == 0) {
     int run = 0;
@@ -327,7 +328,7 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
         if (PAIRS) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (c0 + j < d) o[j] = DT<T>::from_f(acc[i][j]);
+            if (c0 + j < d) reinterpret_cast<float*>(out)[(int64_t)t * d + c0 + j] = acc[i][j];
         } else if (vec_ok) {
           red_add_v4(o, DT<T>::round(acc[i][0]), DT<T>::round(acc[i][1]),
                      DT<T>::round(acc[i][2]), DT<T>::round(acc[i][3]));

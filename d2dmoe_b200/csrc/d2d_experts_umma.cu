@@ -467,7 +467,7 @@ __device__ void role_list(const Params& p, Ctl* c, int lane, bool one_window) {
 // while its rows are copied, and so do the next tile's table words where that tile is known by then.  The
 // selection itself stands between two tiles' copies: a gated expert with two rows per 128-token tile makes it
 // search 64 of those for one of its own.)
-// PAIRS: the list holds pairs token * slots + slot; its rows of out are theirs alone and are stored.
+// PAIRS: the list holds pairs token * slots + slot, and so do the rows of out.
 template <bool PAIRS>
 __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int lane) {
   volatile int* af = &c->abort_flag;
@@ -553,7 +553,7 @@ __device__ void role_gather(const Params& p, Ctl* c, uint32_t ring, int w, int l
     }
     const uint32_t d = __ballot_sync(
         0xffffffffu, __popc(mask[0]) + __popc(mask[1]) + __popc(mask[2]) + __popc(mask[3]) == 1);
-    if (lane == 0) c->tile[q0.s].direct[w] = PAIRS ? 0xffffffffu : d;
+    if (lane == 0) c->tile[q0.s].direct[w] = d;
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(smem_u32(&c->rows_full[q0.s]));
@@ -923,6 +923,87 @@ __device__ void role_drain(const Params& p, Ctl* c, uint32_t tmem, int j, int q4
   }
 }
 
+// The same for lists of pairs, whose rows are stored in the 16-byte pieces of encode8 that a lane has anyway: nothing is
+// exchanged, half lines leave an SM nearly as fast as whole ones (29 to 32 bytes a clock).
+template <bool GLU>
+__device__ void role_drain_pairs(const Params& p, Ctl* c, uint32_t tmem, int j, int q4, int lane) {
+  volatile int* af = &c->abort_flag;
+  const Geo& g = p.g;
+  const int rl = lane >> 2, ql = lane & 3;
+  const bool wide = g.nd == 128;
+  const int col0 = wide ? 64 * j : 0;                // my columns of a step
+  const uint32_t row_bytes = 2 * (uint32_t)p.d;
+  const uint32_t src0 = ((uint32_t)(q4 * 32) << 16) + col0;
+  Acc2Ring<GLU> ar;
+  RingPos q = {0, 0};
+  uint32_t ctx = 0;
+  int turn = wide ? j : 0;                           // group whose step is next
+  for (;; q.next(TILE_RING)) {
+    if (!mbar_wait_warp(smem_u32(&c->tile_full[q.s]), q.ph, af, p.dev_status)) return;
+    const Tile* t = &c->tile[q.s];
+    const int n0 = t->n0, n1 = t->n1;
+    if (t->e < 0) return;
+    if (!mbar_wait_warp(smem_u32(&c->rows_full[q.s]), q.ph, af, p.dev_status)) return;
+    int rt[4];                           // rows rl + 8 i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rt[i] = t->list[q4 * 32 + 8 * i + rl];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c->tile_empty[q.s]));
+    for (int n = n0; n < n1; ++n) {
+      const bool skip = turn != j;
+      if (!wide) turn ^= 1;
+      if (skip) {
+        ar.next(ctx, g.nd);
+        continue;
+      }
+      uint8_t* const o = reinterpret_cast<uint8_t*>(p.out + n * g.nd + col0 + 8 * ql);
+      const uint32_t b = ar.slot(ctx);
+      if (!mbar_wait_warp(smem_u32(&c->acc2_full[b]), ar.at(ctx).ph, af, p.dev_status)) return;
+      tc_fence_after();
+      const uint32_t acc = ar.column(tmem, ctx, g.nd) + src0;
+      ar.next(ctx, g.nd);
+      uint32_t v[32];
+      tmem_ld_frag64(acc, v);
+      tmem_wait_ld32(v);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint4 w[2][2];                   // [row rl + 8 i][block of 32 columns]
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float f[8];
+#pragma unroll
+            for (int h = 0; h < 8; ++h) f[h] = __uint_as_float(v[16 * k + 4 * (h >> 1) + 2 * i + (h & 1)]);
+            w[i][k] = encode8(f);
+          }
+        if (half == 0) tmem_ld_frag64(acc + (16u << 16), v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = rt[2 * half + i];
+          uint8_t* const row = o + (uint64_t)(uint32_t)max(r, 0) * row_bytes;
+          if (r >= 0) {
+            *reinterpret_cast<uint4*>(row) = w[i][0];
+            *reinterpret_cast<uint4*>(row + 64) = w[i][1];
+          }
+        }
+        if (half == 0) {
+          tmem_wait_ld32(v);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&c->acc2_empty[b]));
+        }
+      }
+    }
+    // every read of this tile's tensor memory by this warp is done
+    if (GLU) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c->ctx_free[ctx]));
+    }
+    ctx ^= 1;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // kernel
 // ---------------------------------------------------------------------------
@@ -997,7 +1078,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) experts_tiles_kernel(const Params
   } else if (warp < WARP_GATHER0) {
     const int w = warp - WARP_DRAIN0;
     if constexpr (PAIRS)
-      role_drain<GLU, false, true>(p, c, tmem, w >> 2, w & 3, lane);
+      role_drain_pairs<GLU>(p, c, tmem, w >> 2, w & 3, lane);
     else if (NORM != D2D_NORM_OF_OUTPUT && p.mask_bits)
       role_drain<GLU, false, true>(p, c, tmem, w >> 2, w & 3, lane);
     else

@@ -99,7 +99,8 @@ __device__ __forceinline__ void load_params(const bf16* p, float* f) {
 }
 
 // Sums of M values over the threads of each row.  Rows of more than a warp meet in shared memory, in
-// one of two buffers in turn: a buffer is written again only behind the barrier after its last reads.
+// one of two buffers in turn: a buffer is written again only behind the barrier after its last reads.  The barrier is
+// the row slot's own.
 template <int M>
 __device__ __forceinline__ void row_sum(float (&v)[M], int tpr, float (*buf)[MAX_THREADS / 32][2], int& turn) {
 #pragma unroll 1
@@ -111,14 +112,153 @@ __device__ __forceinline__ void row_sum(float (&v)[M], int tpr, float (*buf)[MAX
   if ((threadIdx.x & 31) == 0)
 #pragma unroll
     for (int m = 0; m < M; ++m) buf[turn][warp][m] = v[m];
-  __syncthreads();
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / tpr), "r"(tpr) : "memory");
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int m = 0; m < M; ++m) v[m] = 0.f;
+  for (int m = 0; m < M; ++m) v[m] = buf[turn][w0 + (lane & (w - 1))][m];
 #pragma unroll 1
-  for (int i = 0; i < w; ++i)
+  for (int o = w >> 1; o > 0; o >>= 1)
 #pragma unroll
-    for (int m = 0; m < M; ++m) v[m] += buf[turn][w0 + i][m];
+    for (int m = 0; m < M; ++m) v[m] += __shfl_xor_sync(0xffffffffu, v[m], o);
   turn ^= 1;
+}
+
+// Rows on their way.  Vectors travel by cp.async into slots that only the thread that asked for them reads, STAGES rows
+// ahead: no barrier, and no register holds them (two rows of registers kept 32 KB in flight on an SM, a third of
+// what DRAM takes to keep up).  Without vectors the next row waits in registers.
+template <int VPT, int IN>                 // IN: inputs (x, and dy)
+constexpr int ring_stages = IN * VPT <= 6 ? 4 : 2;       // (512 threads with eight vectors each: 128 KB)
+template <typename T, int V, int VPT, int IN>
+struct Ahead {
+  static constexpr int STAGES = ring_stages<VPT, IN>;
+  static constexpr bool RING = V > 1;
+  Vec<T, V> next[RING ? 1 : IN][RING ? 1 : VPT];
+  uint4* slots;                            // [STAGES][IN][VPT][threads]
+  int stage = 0;
+  __device__ __forceinline__ uint4* slot(int st, int n, int i) const {
+    return slots + ((st * IN + n) * VPT + i) * (int)blockDim.x + (int)threadIdx.x;
+  }
+  // asks for a row (nothing where it is not there)
+  __device__ __forceinline__ void fetch(int st, const T* const (&row)[IN], bool in, int ti, int tpr, int nv) {
+#pragma unroll
+    for (int n = 0; n < IN; ++n)
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = ti + i * tpr;
+        if constexpr (RING) {
+          if (in && c < nv)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             (uint32_t)__cvta_generic_to_shared(slot(st, n, i))),
+                         "l"(row[n] + (int64_t)c * V)
+                         : "memory");
+        } else {
+          if (in && c < nv) next[n][i].load(row[n] + (int64_t)c * V);
+          else next[n][i].zero();
+        }
+      }
+    if constexpr (RING) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // the row asked for longest ago
+  __device__ __forceinline__ void take(Vec<T, V> (&v)[IN][VPT], bool in, int ti, int tpr, int nv) {
+    if constexpr (RING) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+#pragma unroll
+    for (int n = 0; n < IN; ++n)
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if constexpr (RING) {
+          v[n][i].zero();
+          if (in && ti + i * tpr < nv) v[n][i].load(reinterpret_cast<const T*>(slot(stage, n, i)));
+        } else {
+          v[n][i] = next[n][i];
+        }
+      }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+  static constexpr int DEPTH = RING ? STAGES - 1 : 1;      // rows asked for before the first is taken
+};
+template <int V, int VPT, int IN>
+size_t ahead_bytes(int threads) {
+  return V > 1 ? (size_t)ring_stages<VPT, IN> * IN * VPT * threads * 16 : 0;
+}
+
+// 16-byte words of the backward kernel's parameters: a pair for every two elements of a row's threads
+__host__ __device__ __forceinline__ int scale_words(int tpr, int elements) { return tpr * elements / 4 + 1; }
+
+// Two floats in one instruction: what limits these kernels next to DRAM is the number of instructions (scalar ones, 25 an
+// element, took 42 us for 50432 x 768 forward), and add, mul and fma of pairs round each half as the scalar ones do.
+using pair = unsigned long long;
+__device__ __forceinline__ pair pack2(float lo, float hi) {
+  pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ pair add2(pair a, pair b) {
+  pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair mul2(pair a, pair b) {
+  pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
+  pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// The VPT V elements of a thread in pairs: element k is column column(k).  Without vectors a pair's halves come from
+// two neighbouring turns of the row's threads.
+template <int V>
+__device__ __forceinline__ int column(int k, int ti, int tpr) { return (ti + k / V * tpr) * V + k % V; }
+template <typename T, int V, int VPT>
+__device__ __forceinline__ void to_pairs(const Vec<T, V> (&v)[VPT], pair (&x)[VPT * V / 2]) {
+#pragma unroll
+  for (int k = 0; k < VPT * V; k += 2)
+    x[k / 2] = pack2(v[k / V].get(k % V), v[(k + 1) / V].get((k + 1) % V));
+}
+// zero where there is no column
+template <int V, int VPT>
+__device__ __forceinline__ void cut(pair (&x)[VPT * V / 2], int ti, int tpr, int nv) {
+#pragma unroll
+  for (int k = 0; k < VPT * V; k += 2) {
+    const bool lo = ti + k / V * tpr < nv, hi = ti + (k + 1) / V * tpr < nv;
+    const float2 f = unpack2(x[k / 2]);
+    x[k / 2] = pack2(lo ? f.x : 0.f, hi ? f.y : 0.f);
+  }
+}
+template <typename T, int V, int VPT>
+__device__ __forceinline__ void store_pairs(T* row, const pair (&x)[VPT * V / 2], int ti, int tpr, int nv) {
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (ti + i * tpr >= nv) continue;
+    float f[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const float2 u = unpack2(x[(i * V + q) / 2]);
+      f[q] = (i * V + q) % 2 ? u.y : u.x;
+    }
+    store_vec<V>(row + column<V>(i * V, ti, tpr), f);
+  }
+}
+template <int N>
+__device__ __forceinline__ float sum_pairs(const pair (&x)[N]) {
+  pair a = x[0], b = x[1 % N];
+  if (N > 1) {
+#pragma unroll
+    for (int i = 2; i < N; i += 2) a = add2(a, x[i]);
+#pragma unroll
+    for (int i = 3; i < N; i += 2) b = add2(b, x[i]);
+    a = add2(a, b);
+  }
+  const float2 f = unpack2(a);
+  return f.x + f.y;
 }
 
 // V: elements of a vector (1: rows or parameters that allow no vectors); VPT: vectors of a thread
@@ -127,72 +267,86 @@ __global__ void __launch_bounds__(MAX_THREADS)
 norm_forward_kernel(const T* __restrict__ x, const P* __restrict__ gamma, const P* __restrict__ beta,
                     T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                     const NormShape s) {
+  extern __shared__ __align__(16) uint4 ring[];
   __shared__ float buf[2][MAX_THREADS / 32][2];
+  constexpr int NP = VPT * V / 2;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(x, gamma, beta);
   const int ti = threadIdx.x & (s.tpr - 1), slot = threadIdx.x / s.tpr, rows = blockDim.x / s.tpr;
   const int nv = s.d / V;
+  const bool ragged = nv != s.tpr * VPT;
   const int64_t step = (int64_t)gridDim.x * rows;
   const float inv = 1.f / (float)s.d;
-  Vec<T, V> v[VPT], nxt[VPT];
+  using A = Ahead<T, V, VPT, 1>;
+  A ahead;
+  ahead.slots = ring;
   int turn = 0;
-  auto fetch = [&](Vec<T, V>(&to)[VPT], int64_t row) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = ti + i * s.tpr;
-      if (row < s.N && c < nv) to[i].load(x + row * s.x_stride + (int64_t)c * V);
-      else to[i].zero();
-    }
-  };
   int64_t row = (int64_t)blockIdx.x * rows + slot;
-  fetch(v, row);
-  // (the barrier in row_sum is for the whole block: every row slot takes as many turns)
+  auto fetch = [&](int st, int64_t r) {
+    const T* const at[1] = {x + r * s.x_stride};
+    ahead.fetch(st, at, r < s.N, ti, s.tpr, nv);
+  };
+#pragma unroll
+  for (int i = 0; i < A::DEPTH; ++i) fetch(i, row + i * step);
+  // a thread has the same columns of every row: their parameters stay in registers
+  pair w[NP], b[NP];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float f[V], g[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) f[q] = 1.f, g[q] = 0.f;
+    const int c = column<V>(i * V, ti, s.tpr);
+    if (ti + i * s.tpr < nv) {
+      if (gamma) {
+        load_params<V>(gamma + c, f);
+#pragma unroll
+        for (int q = 0; q < V; ++q) f[q] += s.offset;
+      }
+      if (beta) load_params<V>(beta + c, g);
+    }
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const int k = i * V + q;
+      if (k % 2 == 0) w[k / 2] = pack2(f[q], 0.f), b[k / 2] = pack2(g[q], 0.f);
+      else w[k / 2] = pack2(unpack2(w[k / 2]).x, f[q]), b[k / 2] = pack2(unpack2(b[k / 2]).x, g[q]);
+    }
+  }
+  // (every row slot of a warp takes as many turns: shuffles are for whole warps)
   for (int64_t first = (int64_t)blockIdx.x * rows; first < s.N; first += step, row += step) {
-    fetch(nxt, row + step);
+    const bool in = row < s.N;
+    pair v[NP], acc[2];
+    {
+      Vec<T, V> raw[1][VPT];
+      ahead.take(raw, in, ti, s.tpr, nv);
+      to_pairs(raw[0], v);
+    }
+    fetch(A::RING ? (ahead.stage + A::STAGES - 2) % A::STAGES : 0, row + A::DEPTH * step);
     float mean = 0.f;
     if (s.kind == D2D_NORM_LAYER) {
-      float sum[1] = {0.f};
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum[0] += v[i].get(q);
+      float sum[1] = {sum_pairs(v)};
       row_sum<1>(sum, s.tpr, buf, turn);
       mean = sum[0] * inv;
+      const pair m = pack2(-mean, -mean);
+#pragma unroll
+      for (int k = 0; k < NP; ++k) v[k] = add2(v[k], m);
+      if (ragged) cut<V, VPT>(v, ti, s.tpr, nv);
     }
-    float sq[1] = {0.f};
+    acc[0] = acc[1] = 0;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (ti + i * s.tpr < nv)
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          const float a = v[i].get(q) - mean;
-          sq[0] = fmaf(a, a, sq[0]);
-        }
+    for (int k = 0; k < NP; ++k) acc[k & 1] = fma2(v[k], v[k], acc[k & 1]);
+    float sq[1] = {sum_pairs(acc)};
     row_sum<1>(sq, s.tpr, buf, turn);
     const float rstd = rsqrtf(fmaf(sq[0], inv, s.eps));
-    if (row < s.N) {
-      if (ti == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
-      }
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = ti + i * s.tpr;
-        if (c >= nv) continue;
-        float w[V], b[V], o[V];
-        if (gamma) load_params<V>(gamma + (int64_t)c * V, w);
-        if (beta) load_params<V>(beta + (int64_t)c * V, b);
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          o[q] = (v[i].get(q) - mean) * rstd;
-          if (gamma) o[q] *= w[q] + s.offset;
-          if (beta) o[q] += b[q];
-        }
-        store_vec<V>(y + row * s.d + (int64_t)c * V, o);
-      }
+    if (!in) continue;
+    if (ti == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
     }
+    const pair r = pack2(rstd, rstd);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) v[i] = nxt[i];
+    for (int k = 0; k < NP; ++k) v[k] = fma2(mul2(v[k], r), w[k], b[k]);
+    store_pairs<T, V, VPT>(y + row * s.d, v, ti, s.tpr, nv);
   }
 }
 
@@ -202,90 +356,92 @@ __global__ void __launch_bounds__(MAX_THREADS)
 norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ gamma,
                      const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                      T* __restrict__ dx, float* __restrict__ part, const NormShape s) {
-  extern __shared__ float cols[];            // [row slots of a block][2][d], where a block has several
+  // gamma + offset in fp32 [threads' columns], then rows on their way; at the end [row slots][2][d] column sums
+  extern __shared__ __align__(16) uint4 ring[];
   __shared__ float buf[2][MAX_THREADS / 32][2];
+  constexpr int NP = VPT * V / 2;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(dy, x, gamma, mean_in, rstd_in);
   const int ti = threadIdx.x & (s.tpr - 1), slot = threadIdx.x / s.tpr, rows = blockDim.x / s.tpr;
   const int nv = s.d / V;
   const int64_t step = (int64_t)gridDim.x * rows;
   const float inv = 1.f / (float)s.d;
-  Vec<T, V> a[VPT], b[VPT], an[VPT], bn[VPT];
-  float dg[COLS ? VPT : 1][V], db[COLS ? VPT : 1][V];
+  using A = Ahead<T, V, VPT, 2>;
+  A ahead;
+  ahead.slots = ring + scale_words(s.tpr, VPT * V);
+  int turn = 0;
+  int64_t row = (int64_t)blockIdx.x * rows + slot;
+  auto fetch = [&](int st, int64_t r) {
+    const T* const at[2] = {x + r * s.x_stride, dy + r * s.dy_stride};
+    ahead.fetch(st, at, r < s.N, ti, s.tpr, nv);
+  };
+#pragma unroll
+  for (int i = 0; i < A::DEPTH; ++i) fetch(i, row + i * step);
+  // [pair][thread of a row]: 8 bytes a lane
+  pair* const scale = reinterpret_cast<pair*>(ring);
+  for (int i = threadIdx.x; i < NP * s.tpr; i += blockDim.x) {
+    const int k = 2 * (i / s.tpr), t = i & (s.tpr - 1);
+    const int c0 = column<V>(k, t, s.tpr), c1 = column<V>(k + 1, t, s.tpr);
+    scale[i] = pack2(gamma && c0 < s.d ? DT<P>::to_f(gamma[c0]) + s.offset : 1.f,
+                     gamma && c1 < s.d ? DT<P>::to_f(gamma[c1]) + s.offset : 1.f);
+  }
+  pair dg[COLS ? NP : 1], db[COLS ? NP : 1];
   if (COLS)
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int q = 0; q < V; ++q) dg[i][q] = db[i][q] = 0.f;
-  int turn = 0;
-  auto fetch = [&](Vec<T, V>(&u)[VPT], Vec<T, V>(&w)[VPT], int64_t row) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = ti + i * s.tpr;
-      if (row < s.N && c < nv) {
-        u[i].load(x + row * s.x_stride + (int64_t)c * V);
-        w[i].load(dy + row * s.dy_stride + (int64_t)c * V);
-      } else {
-        u[i].zero();
-        w[i].zero();
-      }
-    }
-  };
-  int64_t row = (int64_t)blockIdx.x * rows + slot;
-  fetch(a, b, row);
+    for (int k = 0; k < NP; ++k) dg[k] = db[k] = 0;
+  float mean = row < s.N && mean_in ? __ldg(mean_in + row) : 0.f, rstd = row < s.N ? __ldg(rstd_in + row) : 0.f;
+  __syncthreads();
   for (int64_t first = (int64_t)blockIdx.x * rows; first < s.N; first += step, row += step) {
-    fetch(an, bn, row + step);
-    const bool in = row < s.N;
-    const float mean = in && mean_in ? __ldg(mean_in + row) : 0.f, rstd = in ? __ldg(rstd_in + row) : 0.f;
-    float sums[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = ti + i * s.tpr;
-      if (c >= nv) continue;
-      float w[V];
-      if (gamma) load_params<V>(gamma + (int64_t)c * V, w);
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const float xh = (a[i].get(q) - mean) * rstd, g = gamma ? b[i].get(q) * (w[q] + s.offset) : b[i].get(q);
-        sums[0] += g;
-        sums[1] = fmaf(g, xh, sums[1]);
-        if (COLS && in) {                    // (a row that is not there has no say, whatever x's first rows hold)
-          dg[i][q] = fmaf(b[i].get(q), xh, dg[i][q]);
-          db[i][q] += b[i].get(q);
-        }
-      }
+    const bool in = row < s.N, more = row + step < s.N;
+    pair xh[NP], g[NP], acc[2];
+    {
+      Vec<T, V> raw[2][VPT];
+      ahead.take(raw, in, ti, s.tpr, nv);
+      to_pairs(raw[0], xh);
+      to_pairs(raw[1], g);
     }
+    fetch(A::RING ? (ahead.stage + A::STAGES - 2) % A::STAGES : 0, row + A::DEPTH * step);
+    const float mean1 = more && mean_in ? __ldg(mean_in + row + step) : 0.f,
+                rstd1 = more ? __ldg(rstd_in + row + step) : 0.f;
+    // (a row or column that is not there is zero, and so is its dy: it adds nothing)
+    const pair r = pack2(rstd, rstd), m = pack2(-mean, -mean);
+    acc[0] = acc[1] = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      xh[k] = mul2(add2(xh[k], m), r);
+      if (COLS) {
+        dg[k] = fma2(g[k], xh[k], dg[k]);
+        db[k] = add2(db[k], g[k]);
+      }
+      g[k] = mul2(g[k], scale[k * s.tpr + ti]);
+      acc[k & 1] = fma2(g[k], xh[k], acc[k & 1]);
+    }
+    float sums[2] = {s.kind == D2D_NORM_LAYER ? sum_pairs(g) : 0.f, sum_pairs(acc)};
     row_sum<2>(sums, s.tpr, buf, turn);
-    const float m0 = s.kind == D2D_NORM_LAYER ? sums[0] * inv : 0.f, m1 = sums[1] * inv;
     if (in && dx) {
+      const float m0 = -sums[0] * inv * rstd, m1 = -sums[1] * inv * rstd;
+      const pair m02 = pack2(m0, m0), m12 = pack2(m1, m1);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = ti + i * s.tpr;
-        if (c >= nv) continue;
-        float w[V], o[V];
-        if (gamma) load_params<V>(gamma + (int64_t)c * V, w);
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-          const float xh = (a[i].get(q) - mean) * rstd, g = gamma ? b[i].get(q) * (w[q] + s.offset) : b[i].get(q);
-          o[q] = rstd * (g - m0 - xh * m1);
-        }
-        store_vec<V>(dx + row * s.d + (int64_t)c * V, o);
-      }
+      for (int k = 0; k < NP; ++k) g[k] = fma2(xh[k], m12, fma2(g[k], r, m02));
+      store_pairs<T, V, VPT>(dx + row * s.d, g, ti, s.tpr, nv);
     }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) a[i] = an[i], b[i] = bn[i];
+    mean = mean1;
+    rstd = rstd1;
   }
   if (!COLS) return;
+  if (A::RING) asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();                           // (the ring is over)
+  float* const cols = reinterpret_cast<float*>(ring);
   float* const mine = rows > 1 ? cols + (int64_t)slot * 2 * s.d : part + (int64_t)blockIdx.x * 2 * s.d;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = ti + i * s.tpr;
-    if (c < nv)
-#pragma unroll
-      for (int q = 0; q < V; ++q) {
-        mine[c * V + q] = dg[i][q];
-        mine[s.d + c * V + q] = db[i][q];
-      }
+  for (int k = 0; k < VPT * V; ++k) {
+    const int c = column<V>(k, ti, s.tpr);
+    const float2 u = unpack2(dg[COLS ? k / 2 : 0]), v = unpack2(db[COLS ? k / 2 : 0]);
+    if (c < s.d) {
+      mine[c] = k % 2 ? u.y : u.x;
+      mine[s.d + c] = k % 2 ? v.y : v.x;
+    }
   }
   if (rows > 1) {
     __syncthreads();
@@ -297,24 +453,26 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const P*
   }
 }
 
-// dgamma and dbeta from the partial rows: 32 columns and eight parts of the rows per block
+// dgamma and dbeta from the partial rows: 32 columns and as many parts of the rows per block
+constexpr int COLUMN_WARPS = 32;
 template <typename P>
-__global__ void __launch_bounds__(BLOCK)
+__global__ void __launch_bounds__(32 * COLUMN_WARPS)
 norm_columns_kernel(const float* __restrict__ part, int blocks, int d, P* __restrict__ dgamma,
                     P* __restrict__ dbeta) {
-  __shared__ float sums[BLOCK / 32][32];
+  __shared__ float sums[COLUMN_WARPS][32];
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(part);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float sum = 0.f;
   if (c < 2 * d)
-#pragma unroll 8
-    for (int b = w; b < blocks; b += BLOCK / 32) sum += part[(int64_t)b * 2 * d + c];
+#pragma unroll 10
+    for (int b = w; b < blocks; b += COLUMN_WARPS) sum += part[(int64_t)b * 2 * d + c];
   sums[w][lane] = sum;
   __syncthreads();
   if (w != 0 || c >= 2 * d) return;
 #pragma unroll
-  for (int i = 1; i < BLOCK / 32; ++i) sum += sums[i][lane];
+  for (int i = 1; i < COLUMN_WARPS; ++i) sum += sums[i][lane];
   P* const to = c < d ? dgamma : dbeta;
   if (to) to[c < d ? c : c - d] = DT<P>::from_f(sum);
 }
@@ -337,9 +495,12 @@ template <typename T, typename P, int V, int VPT>
 int forward_vpt(const T* x, const P* gamma, const P* beta, T* y, float* mean, float* rstd, NormShape s,
                 int sms, cudaStream_t st) {
   const int threads = s.tpr > BLOCK ? s.tpr : BLOCK, rows = threads / s.tpr;
-  const int grid = blocks_for(s.N, rows, sms, 1024 / threads);
-  return launch_pdl(norm_forward_kernel<T, P, V, VPT>, dim3((unsigned)grid), dim3((unsigned)threads), 0,
-                    st, x, gamma, beta, y, mean, rstd, s);
+  const size_t smem = ahead_bytes<V, VPT, 1>(threads);
+  const auto k = norm_forward_kernel<T, P, V, VPT>;
+  const int rc = device_launch_facts((const void*)k, smem, nullptr);
+  if (rc != D2D_OK) return rc;
+  const int grid = blocks_for(s.N, rows, sms, (VPT * V > 16 ? 512 : 1024) / threads);      // what is resident at once
+  return launch_pdl(k, dim3((unsigned)grid), dim3((unsigned)threads), smem, st, x, gamma, beta, y, mean, rstd, s);
 }
 
 template <typename T, typename P>
@@ -349,7 +510,7 @@ int forward_t(const T* x, const P* gamma, const P* beta, T* y, float* mean, floa
   const bool vec = s.d % VW == 0 && (s.x_stride * (int64_t)sizeof(T)) % 16 == 0 && aligned16(x) &&
                    aligned16(y) && aligned16(gamma) && aligned16(beta);
   int nv = s.d / VW;
-  if (vec) s.tpr = threads_per_row(nv, nv <= 32 ? 1 : nv <= 96 ? 3 : nv <= 256 ? 2 : 4);
+  if (vec) s.tpr = threads_per_row(nv, nv <= 64 ? 2 : nv <= 96 ? 3 : 4);
   if (vec && s.tpr != 0) {
     const int vpt = ceil_div(nv, s.tpr);
     return vpt <= 1   ? forward_vpt<T, P, VW, 1>(x, gamma, beta, y, mean, rstd, s, sms, st)
@@ -372,19 +533,19 @@ int backward_vpt(const T* dy, const T* x, const P* gamma, const float* mean, con
                  P* dgamma, P* dbeta, float* part, NormShape s, int sms, cudaStream_t st) {
   const int threads = s.tpr > BLOCK ? s.tpr : BLOCK, rows = threads / s.tpr;
   const bool cols = dgamma || dbeta;
-  if (!cols)
-    return launch_pdl(norm_backward_kernel<T, P, V, VPT, false>,
-                      dim3((unsigned)blocks_for(s.N, rows, sms, 1024 / threads)), dim3((unsigned)threads), 0,
-                      st, dy, x, gamma, mean, rstd, dx, part, s);
-  const size_t smem = rows > 1 ? (size_t)rows * 2 * s.d * sizeof(float) : 0;
-  const auto k = norm_backward_kernel<T, P, V, VPT, true>;
+  const size_t in_flight = ahead_bytes<V, VPT, 2>(threads) + (size_t)scale_words(s.tpr, VPT * V) * 16;
+  const size_t smem = cols && rows > 1 ? std::max(in_flight, (size_t)rows * 2 * s.d * sizeof(float)) : in_flight;
+  const auto k = cols ? norm_backward_kernel<T, P, V, VPT, true> : norm_backward_kernel<T, P, V, VPT, false>;
   int rc = device_launch_facts((const void*)k, smem, nullptr);
   if (rc != D2D_OK) return rc;
-  const int grid = std::min(blocks_for(s.N, rows, sms, 2), PARTIAL_BLOCKS);
+  if (!cols)
+    return launch_pdl(k, dim3((unsigned)blocks_for(s.N, rows, sms, 1024 / threads)), dim3((unsigned)threads), smem, st,
+                      dy, x, gamma, mean, rstd, dx, part, s);
+  const int grid = std::min(blocks_for(s.N, rows, sms, 512 / threads), PARTIAL_BLOCKS);
   rc = launch_pdl(k, dim3((unsigned)grid), dim3((unsigned)threads), smem, st, dy, x, gamma, mean, rstd, dx,
                   part, s);
   if (rc != D2D_OK) return rc;
-  return launch_pdl(norm_columns_kernel<P>, dim3((unsigned)ceil_div(2 * s.d, 32)), dim3(BLOCK), 0, st,
+  return launch_pdl(norm_columns_kernel<P>, dim3((unsigned)ceil_div(2 * s.d, 32)), dim3(32 * COLUMN_WARPS), 0, st,
                     (const float*)part, grid, s.d, dgamma, dbeta);
 }
 
@@ -396,7 +557,7 @@ int backward_t(const T* dy, const T* x, const P* gamma, const float* mean, const
                    (s.dy_stride * (int64_t)sizeof(T)) % 16 == 0 && aligned16(x) && aligned16(dy) &&
                    aligned16(dx) && aligned16(gamma);
   int nv = s.d / VW;
-  if (vec) s.tpr = threads_per_row(nv, nv <= 32 ? 1 : nv <= 96 ? 3 : nv <= 1024 ? 2 : 4);
+  if (vec) s.tpr = threads_per_row(nv, nv <= 64 ? 2 : nv <= 96 ? 3 : nv <= 1024 ? 2 : 4);
   if (vec && s.tpr != 0) {
     const int vpt = ceil_div(nv, s.tpr);
     return vpt <= 1   ? backward_vpt<T, P, VW, 1>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)

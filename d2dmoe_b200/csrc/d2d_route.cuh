@@ -47,6 +47,7 @@ struct RouteArgs {
   bool softmax, renormalise;
   float scale;
   int room;                                // shared memory of a warp, bytes
+  bool bias_vectors;                       // the bias allows 16-byte loads
   uint32_t group_magic;                    // e group_magic >> 22 = e / (E / groups) for e < 1024
 };
 
@@ -58,6 +59,11 @@ constexpr float LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 // e^(l - m): 2 ulp and |l - m| half ulps off
@@ -226,10 +232,11 @@ __device__ __noinline__ void route_exact(const RouteArgs& a, int64_t t, double* 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT) route_exact_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(NT) route_exact_kernel(RouteArgs a) {
   extern __shared__ __align__(16) double scratch[];
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(a.logits, a.bias);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t t = (int64_t)blockIdx.x * WARPS + warp; t < a.N; t += (int64_t)gridDim.x * WARPS)
     route_exact<T>(a, t, scratch + (size_t)warp * a.E, lane);
@@ -375,12 +382,13 @@ __device__ __forceinline__ float2 two_best(const float* c) {
 
 // L lanes per token, EL logits per lane, lists of KP keys; V logits per load.
 template <typename T, int V, int L, int EL, int KP, int MODE>
-__global__ void __launch_bounds__(NT, MODE == ORDER && KP == 8 ? 6 : 4) route_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ? 6 : 8) : EL == 32 ? 4 : MODE == TOTAL ? 8 : 6) route_kernel(RouteArgs a) {
   extern __shared__ __align__(16) double scratch[];
   constexpr int TOKENS = 32 / L;           // of a warp at once
   constexpr int R = (KP + L - 1) / L;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(a.logits, a.bias);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane % L, mine = lane / L;
   const int E = a.E, k = a.k;
   double* const wide = scratch + (size_t)warp * (a.room / 8);
@@ -420,16 +428,30 @@ __global__ void __launch_bounds__(NT, MODE == ORDER && KP == 8 ? 6 : 4) route_ke
       } else {
 #pragma unroll
         for (int i = 0; i < EL; ++i)
-          c[i] = __fdividef(1.f, 1.f + exp2_fast(fminf(row.get(i) * -LOG2E, 120.f)));
+          c[i] = reciprocal_fast(1.f + exp2_fast(fminf(row.get(i) * -LOG2E, 120.f)));
       }
       if (a.bias) {
         float worst = 0.f;
 #pragma unroll
-        for (int i = 0; i < EL; ++i) {
-          const int e = row.expert(i, q);
-          const float b = e < E ? __ldg(a.bias + e) : 0.f;
-          worst = max_nan(worst, b);
-          c[i] += b;
+        for (int v = 0; v < EL / V; ++v) {
+          const int e = (v * L + q) * V;
+          if (e >= E) continue;
+          float b[V];
+          if (V > 1 && a.bias_vectors) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+              const float4 x = __ldg(reinterpret_cast<const float4*>(a.bias + e) + i);
+              b[4 * i] = x.x, b[4 * i + 1] = x.y, b[4 * i + 2] = x.z, b[4 * i + 3] = x.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) b[i] = __ldg(a.bias + e + i);
+          }
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            worst = max_nan(worst, b[i]);
+            c[v * V + i] += b[i];
+          }
         }
         bad |= unusable(max_lanes<L>(worst));
       }
@@ -642,11 +664,12 @@ struct BackwardArgs {
 };
 
 template <typename T, int V, int L, int EL>
-__global__ void __launch_bounds__(NT) route_backward_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(NT) route_backward_kernel(BackwardArgs a) {
   extern __shared__ __align__(16) double scratch[];
   constexpr int TOKENS = 32 / L;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(a.logits, a.experts, a.weights, a.dweights);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane % L, mine = lane / L;
   const int E = a.E, EP = (E + 3) / 4 * 4;
   float* const share = reinterpret_cast<float*>(scratch) + (size_t)(warp * TOKENS + mine) * EP;

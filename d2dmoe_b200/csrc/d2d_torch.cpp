@@ -827,16 +827,20 @@ PyObject* experts_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   if (k < 1 || k > E) return PyLong_FromLong(D2D_ERR_BAD_ARG);
   On on(xt);
-  const at::Tensor x = xt.contiguous(), e = et.contiguous(), w = wt.contiguous();
+  const auto aligned = [](at::Tensor t) {      // (views may start anywhere)
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+  };
+  const at::Tensor x = aligned(xt.contiguous()), e = et.contiguous(), w = wt.contiguous();
+  const at::Tensor lb = bias ? aligned(*bias) : at::Tensor();
   at::Tensor out = at::detail::empty_cuda(xt.sizes(), xt.options()), ws;
   size_t bytes = 0;
-  int rc = d2d_experts_weighted_workspace_bytes(N, (int)d, (int)E, (int)H, (int)k, up != nullptr, dt, &bytes);
+  int rc = d2d_experts_weighted_workspace_bytes(N, (int)d, (int)E, (int)H, (int)k, up != nullptr, packed != nullptr, dt, &bytes);
   if (rc != D2D_OK) return PyLong_FromLong(rc);
   if (N > 0) {
     ws = at::detail::empty_cuda({(int64_t)bytes}, xt.options().dtype(at::kByte));
     rc = d2d_experts_weighted(x.data_ptr(), (const int32_t*)e.data_ptr(), (const float*)w.data_ptr(), w1.data_ptr(),
                               data_or_null(b1), data_or_null(up), w2.data_ptr(), data_or_null(packed),
-                              data_or_null(bias), residual, out.data_ptr(), N, (int)d, (int)E, (int)H, (int)k, act, dt,
+                              data_or_null(&lb), residual, out.data_ptr(), N, (int)d, (int)E, (int)H, (int)k, act, dt,
                               ws.data_ptr(), bytes, (int*)data_or_null(status), on.stream);
   }
   if (rc != D2D_OK) return PyLong_FromLong(rc);

@@ -24,7 +24,7 @@ int launch_experts_umma(const void* x, int32_t* token_idx, int32_t* offsets,
                         const MaskTable* mt = nullptr);
 
 // Lists of pairs p = token k + slot (k: slots per token): out is [N k, d], row p is stored and is the expert's output for the
-// token; the hidden values are rounded once
+// token, in 16-byte pieces of eight columns (encode8); the hidden values are rounded once
 int launch_experts_umma_pairs(const void* x, int32_t* pairs, int32_t* offsets, const void* packed, void* out,
                               int64_t N, int d, int E, int H, int k, bool glu, int act, int* dev_status,
                               cudaStream_t s);

@@ -6,92 +6,121 @@
 // taken in the order of its slots and rounded once, so a call gives the same bits every time.  Two ways:
 //   lists   The pairs p = t k + j are sorted by expert (counting sort, ascending p in each list), the expert kernels
 //           run over the lists and store row p of a table [N k, d], and a last pass sums each token's k rows, which
-//           lie together.  The table is in T: a row is rounded once more than it would have to be, which costs as
-//           much accuracy as the rounding of the tensor cores' hidden operand does (2^-9 of a row's size in
-//           bf16); rows of 32 bits would double the traffic that bounds this form.
+//           lie together.  That table is what bounds this form: it is written and read once (50432 tokens x 4 x 768:
+//           310 MB each way next to 155 MB of x and out).  The tensor-core kernel's rows are 16 bits an
+//           element, in a format of its own (encode8) that is off by 2^-14 of the largest of eight where bf16 would be by 2^-9; the
+//           general-shape kernel's are fp32.
 //   few     Calls of few pairs are bound by latency and by the weights' bytes: two kernels without lists, all
 //           sums in 32 bits.  The first splits every pair's hidden columns and, where there are fewer such pieces than SMs,
 //           the depth d over blocks; the second adds the depth's parts, applies bias, activation and weight, and takes
-//           the second product over all k H hidden values of a token at once.
+//           the second product, the slots of a token split over a cluster whose sums meet in distributed shared memory.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
-#include "d2d_common.cuh"
-#include "d2d_umma_api.cuh"
+#include "d2d_experts_common.cuh"
 
 namespace d2d {
 namespace {
 
 constexpr int NT = 256;
 constexpr int MAX_E = 256;
-constexpr int64_t ONE_BLOCK_PAIRS = 4096;   // sorted by a single block of 1024 threads
-constexpr int CHUNK_BLOCKS = 148;           // blocks of larger sorts, at most
 
 // -- lists of pairs ---------------------------------------------------------------------------------
 // Counting sort, stable: every block counts its chunk of the pairs (the first kernel), then, knowing everyone's counts,
-// writes it: warps take contiguous parts of the chunk, 32 pairs at a time, and pairs of one expert among them
-// rank by lane.
+// writes it: warps take contiguous parts of the chunk, and pairs of one expert among 32 neighbours rank by lane.  A
+// thread's R pairs are loaded at once and stay in registers; calls of one chunk need the second kernel only.
+// The table of counts: [blocks][EP], EP = E up to a multiple of 8, 16 bits each (a chunk has 4096 pairs at most).
+template <int R>
+__device__ __forceinline__ void load_pairs(const int32_t* __restrict__ experts, int64_t p0, int64_t P, int E, int lane,
+                                           int (&e)[R], int* dev_status) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) e[i] = p0 + 32 * i + lane < P ? experts[p0 + 32 * i + lane] : -1;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if ((unsigned)e[i] >= (unsigned)E) {
+      if (e[i] != -1) report(dev_status, D2D_ERR_INDEX_RANGE);
+      e[i] = -1;
+    }
+}
+
+template <int R>
 __global__ void __launch_bounds__(NT)
-pairs_count_kernel(const int32_t* __restrict__ experts, int64_t P, int E, int64_t chunk,
-                   int32_t* __restrict__ table) {
+pairs_count_kernel(const int32_t* __restrict__ experts, int64_t P, int E, int EP, uint16_t* __restrict__ table) {
   __shared__ int hist[MAX_E];
   grid_launch_dependents();
   grid_dependency_wait();
-  for (int e = threadIdx.x; e < E; e += NT) hist[e] = 0;
+  fresh(experts);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int e[R];
+  load_pairs<R>(experts, ((int64_t)blockIdx.x * (NT / 32) + w) * 32 * R, P, E, lane, e, nullptr);
+  for (int i = threadIdx.x; i < EP; i += NT) hist[i] = 0;
   __syncthreads();
-  const int64_t p0 = blockIdx.x * chunk, p1 = min(P, p0 + chunk);
-  for (int64_t p = p0 + threadIdx.x; p < p1; p += NT) {
-    const int e = experts[p];
-    if ((unsigned)e < (unsigned)E) atomicAdd(&hist[e], 1);
-  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (e[i] >= 0) atomicAdd(&hist[e[i]], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += NT) table[(int64_t)blockIdx.x * E + e] = hist[e];
+  for (int i = threadIdx.x; i < EP; i += NT) table[(int64_t)blockIdx.x * EP + i] = (uint16_t)hist[i];
 }
 
-// one block: no table.  Shared memory: [warps][E], then 3 E + 1 words.
-__global__ void __launch_bounds__(1024)
-pairs_scatter_kernel(const int32_t* __restrict__ experts, int64_t P, int E, int64_t chunk,
-                     const int32_t* __restrict__ table, int32_t* __restrict__ pairs,
-                     int32_t* __restrict__ offsets, int* dev_status) {
-  extern __shared__ int sm[];
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, warps = blockDim.x >> 5;
-  int* const mine = sm + w * E;             // this warp's counts, then where its next pair of an expert goes
-  int* const total = sm + warps * E;        // [E]
-  int* const before = total + E;            // [E]: pairs of earlier blocks
-  int* const first = before + E;            // [E + 1]
+// table null: one block
+template <int R>
+__global__ void __launch_bounds__(NT)
+pairs_scatter_kernel(const int32_t* __restrict__ experts, int64_t P, int E, int EP, const uint16_t* __restrict__ table,
+                     int32_t* __restrict__ pairs, int32_t* __restrict__ offsets, int* dev_status) {
+  constexpr int WARPS = NT / 32;
+  __shared__ int count[WARPS][MAX_E];       // a warp's pairs of each expert, then where its next one goes
+  __shared__ int total[MAX_E], before[MAX_E], first[MAX_E + 1];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   grid_launch_dependents();
-  grid_dependency_wait();
-  for (int i = tid; i < warps * E + 2 * E; i += blockDim.x) sm[i] = 0;
-  __syncthreads();
-  const int64_t part = (chunk + warps - 1) / warps;
-  const int64_t p0 = blockIdx.x * chunk + w * part, p1 = min(min(P, (blockIdx.x + 1) * chunk), p0 + part);
-  for (int64_t p = p0 + lane; p < p1; p += 32) {
-    const int e = experts[p];
-    if ((unsigned)e < (unsigned)E) atomicAdd(&mine[e], 1);
-    else if (e != -1) report(dev_status, D2D_ERR_INDEX_RANGE);
+  for (int i = tid; i < MAX_E; i += NT) {
+    total[i] = before[i] = 0;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) count[v][i] = 0;
   }
+  grid_dependency_wait();
+  fresh(experts, table);
+  const int64_t p0 = ((int64_t)blockIdx.x * WARPS + w) * 32 * R;
+  int e[R];
+  load_pairs<R>(experts, p0, P, E, lane, e, dev_status);
   __syncthreads();
-  if (table) {
-    int EP = 1;
-    while (EP < E) EP *= 2;
-    const int e = tid & (EP - 1), parts = blockDim.x / EP;
-    int all = 0, early = 0;
-    if (e < E)
+  if (table) {                              // eight experts a thread, as many rows at once as there are threads
+    const int per = EP / 8, g = tid % per, rows = NT / per;
+    int all[8], early[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all[i] = early[i] = 0;
+    if (tid < rows * per)
 #pragma unroll 4
-      for (int b = tid / EP; b < (int)gridDim.x; b += parts) {
-        const int n = table[(int64_t)b * E + e];
-        all += n;
-        early += b < (int)blockIdx.x ? n : 0;
+      for (int b = tid / per; b < (int)gridDim.x; b += rows) {
+        const uint4 v = *reinterpret_cast<const uint4*>(table + (int64_t)b * EP + 8 * g);
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+        const bool mine = b < (int)blockIdx.x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = (int)(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu);
+          all[i] += n;
+          early[i] += mine ? n : 0;
+        }
       }
-    if (all) atomicAdd(&total[e], all);
-    if (early) atomicAdd(&before[e], early);
-  } else {
-    for (int e = tid; e < E; e += blockDim.x) {
-      int sum = 0;
-      for (int i = 0; i < warps; ++i) sum += sm[i * E + e];
-      total[e] = sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (all[i]) atomicAdd(&total[8 * g + i], all[i]);
+      if (early[i]) atomicAdd(&before[8 * g + i], early[i]);
     }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (e[i] >= 0) atomicAdd(&count[w][e[i]], 1);
   __syncthreads();
+  if (!table) {
+    for (int i = tid; i < E; i += NT) {
+      int sum = 0;
+#pragma unroll
+      for (int v = 0; v < WARPS; ++v) sum += count[v][i];
+      total[i] = sum;
+    }
+    __syncthreads();
+  }
   if (w == 0) {
     int run = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
@@ -109,27 +138,27 @@ pairs_scatter_kernel(const int32_t* __restrict__ experts, int64_t P, int E, int6
   }
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int e = tid; e <= E; e += blockDim.x) offsets[e] = first[e];
-  for (int e = tid; e < E; e += blockDim.x) {
-    int run = first[e] + before[e];
-    for (int i = 0; i < warps; ++i) {
-      const int n = sm[i * E + e];
-      sm[i * E + e] = run;
+    for (int i = tid; i <= E; i += NT) offsets[i] = first[i];
+  for (int i = tid; i < E; i += NT) {
+    int run = first[i] + before[i];
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      const int n = count[v][i];
+      count[v][i] = run;
       run += n;
     }
   }
   __syncthreads();
-  for (int64_t q = p0; q < p1; q += 32) {
-    const int64_t p = q + lane;
-    int e = p < p1 ? experts[p] : -1;
-    if ((unsigned)e >= (unsigned)E) e = -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
+  int* const mine = count[w];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const uint32_t same = __match_any_sync(0xffffffffu, e[i]);
     int at = 0;
-    if (e >= 0) at = mine[e] + __popc(same & ((1u << lane) - 1u));
+    if (e[i] >= 0) at = mine[e[i]] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
-    if (e >= 0) {
-      pairs[at] = (int)p;
-      if ((same >> lane) == 1u) mine[e] = at + 1;      // the last of them
+    if (e[i] >= 0) {
+      pairs[at] = (int)(p0 + 32 * i + lane);
+      if ((same >> lane) == 1u) mine[e[i]] = at + 1;      // the last of them
     }
     __syncwarp();
   }
@@ -165,44 +194,73 @@ __device__ __forceinline__ void store_row(T* p, const float* f) {
   }
 }
 
-// y: [N k, d].  A warp has a token; its weights are in its lanes.
-template <typename T, int V>
+// y: [N k, d] fp32 or (CODED) in pieces of encode8.  A thread has V columns of a token; a block takes a few tokens.
+template <typename T, int V, bool CODED>
 __global__ void __launch_bounds__(NT)
-combine_kernel(const T* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
+combine_kernel(const void* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
                const T* __restrict__ last_bias, const T* __restrict__ x, T* __restrict__ out, int64_t N, int d,
-               int E, int k) {
+               int E, int k, int tokens) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, nv = d / V;
-  for (int64_t t = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5); t < N; t += (int64_t)gridDim.x * (NT / 32)) {
-    const int e = lane < k ? experts[t * k + lane] : -1;
-    const float w = lane < k ? weights[t * k + lane] : 0.f;
-    const uint32_t there = __ballot_sync(0xffffffffu, (unsigned)e < (unsigned)E);
-    for (int c = lane; c < ceil_div(nv, 32) * 32; c += 32) {
-      float sum[V], f[V];
+  fresh(y, experts, weights, last_bias, x);
+  const int nv = d / V;
+  const int64_t t0 = (int64_t)blockIdx.x * tokens;
+  const int items = (int)min((int64_t)tokens, N - t0) * nv;
+  for (int i = threadIdx.x; i < items; i += NT) {
+    const int dt = i / nv, c = (i - dt * nv) * V;
+    const int64_t t = t0 + dt;
+    float sum[V], f[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < k; ++j) {
-        const float wj = __shfl_sync(0xffffffffu, w, j);
-        if ((there >> j & 1u) == 0u || c >= nv) continue;
-        load_row<T, V>(y + (t * k + j) * d + (int64_t)c * V, f);
+    for (int q = 0; q < V; ++q) sum[q] = 0.f;
+    // (four rows' loads at a time, asked for before the first is used)
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      uint4 raw[4];
+      float4 lo[4], hi[4];
+      float wt[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = fmaf(wj, f[i], sum[i]);
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u;
+        const int e = j < k ? __ldg(experts + t * k + j) : -1;
+        wt[u] = 0.f;
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if ((unsigned)e < (unsigned)E) {
+          wt[u] = __ldg(weights + t * k + j);
+          const int64_t at = (t * k + j) * d + c;
+          if constexpr (CODED) {
+            raw[u] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(y) + at));
+          } else {
+            const float* p = reinterpret_cast<const float*>(y) + at;
+            if constexpr (V == 1) lo[u].x = __ldg(p);
+            if constexpr (V >= 4) lo[u] = __ldg(reinterpret_cast<const float4*>(p));
+            if constexpr (V == 8) hi[u] = __ldg(reinterpret_cast<const float4*>(p) + 1);
+          }
+        } else {
+          wt[u] = 0.f;
+        }
       }
-      if (c >= nv) continue;
-      if (last_bias) {
-        load_row<T, V>(last_bias + (int64_t)c * V, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += f[i];
-      }
-      if (x) {
-        load_row<T, V>(x + t * d + (int64_t)c * V, f);
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (CODED) {
+          if (j0 + u < k) umma::add_decoded8(raw[u], wt[u], sum);      // (no expert: zeros of weight zero)
+        } else {
+          const float v[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += f[i];
+          for (int q = 0; q < V; ++q) sum[q] = fmaf(wt[u], v[q], sum[q]);
+        }
       }
-      store_row<T, V>(out + t * d + (int64_t)c * V, sum);
     }
+    if (last_bias) {
+      load_row<T, V>(last_bias + c, f);
+#pragma unroll
+      for (int q = 0; q < V; ++q) sum[q] += f[q];
+    }
+    if (x) {
+      load_row<T, V>(x + t * d + c, f);
+#pragma unroll
+      for (int q = 0; q < V; ++q) sum[q] += f[q];
+    }
+    store_row<T, V>(out + t * d + c, sum);
   }
 }
 
@@ -235,11 +293,12 @@ __device__ __forceinline__ float few_sum(float (&v)[V], float* red) {
 // part[s][p][gate, up][H]: pair p's share of x W1 (and x W_up) from depth part s
 template <typename T, int V, bool GLU>
 __global__ void __launch_bounds__(NT)
-few_hidden_kernel(const WeightedCall c, int splits, float* __restrict__ part) {
+few_hidden_kernel(WeightedCall c, int splits, float* __restrict__ part) {
   constexpr int TC = few_threads<V>, RG = NT / TC, G = GLU ? 2 : 1;
   __shared__ float red[NT / 32 * TC * V];
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(c.x, c.experts, c.w1, c.w_up);
   const int tid = threadIdx.x, H = c.H, d = c.d;
   const int hcs = ceil_div(H, TC * V), hc = blockIdx.x % hcs, s = blockIdx.x / hcs;
   const int64_t p = blockIdx.y, P = c.N * c.k, t = p / c.k;
@@ -281,67 +340,77 @@ few_hidden_kernel(const WeightedCall c, int splits, float* __restrict__ part) {
   }
 }
 
+// A cluster has V few_threads columns of a token, a CTA of it `share` slots: blockIdx.x = (columns, CTA of the cluster).
 template <typename T, int V, bool GLU>
 __global__ void __launch_bounds__(NT)
-few_out_kernel(const WeightedCall c, int splits, const float* __restrict__ part) {
+few_out_kernel(WeightedCall c, int splits, int share, const float* __restrict__ part) {
   constexpr int TC = few_threads<V>, RG = NT / TC, G = GLU ? 2 : 1;
-  extern __shared__ float hs[];             // [k][H] hidden values times their weight, then [k] experts
+  extern __shared__ float hs[];             // [share][H] hidden values times their weight, then [share] experts
   __shared__ float red[NT / 32 * TC * V];
+  __shared__ float sums[TC * V];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, H = c.H, d = c.d, k = c.k;
-  int* const es = reinterpret_cast<int*>(hs + k * H);
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int j0 = rank * share, js = max(0, min(share, k - j0));          // my slots
+  int* const es = reinterpret_cast<int*>(hs + share * H);
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(c.x, c.experts, c.weights, c.b1, c.w2, c.last_bias, part);
   const int64_t t = blockIdx.y, P = c.N * k;
-  for (int j = tid; j < k; j += NT) {
-    const int e = c.experts[t * k + j];
+  for (int j = tid; j < js; j += NT) {
+    const int e = c.experts[t * k + j0 + j];
     es[j] = (unsigned)e < (unsigned)c.E ? e : -1;
   }
   __syncthreads();
-  for (int i = tid; i < k * H; i += NT) {
+  for (int i = tid; i < js * H; i += NT) {
     const int j = i / H, h = i - j * H, e = es[j];
     float v = 0.f;
     if (e >= 0) {
-      const float* q = part + (t * k + j) * G * H + h;
+      const float* q = part + (t * k + j0 + j) * G * H + h;
       float up = 0.f;
-      for (int s = 0; s < splits; ++s, q += P * G * H) {
-        v += q[0];
-        if (GLU) up += q[H];
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) {
+        v += q[s * P * G * H];
+        if (GLU) up += q[s * P * G * H + H];
       }
       if (c.b1) v += DT<T>::to_f(((const T*)c.b1)[(int64_t)e * H + h]);
       v = activate(v, c.act);
       if (GLU) v *= up;
-      v *= c.weights[t * k + j];
+      v *= c.weights[t * k + j0 + j];
     }
     hs[i] = v;
   }
   __syncthreads();
-  const int col = blockIdx.x * TC * V + (tid % TC) * V;
+  const int col0 = blockIdx.x / ctas * TC * V, col = col0 + (tid % TC) * V;
   float a[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) a[i] = 0.f;
-  if (col < d) {
-    int j = 0, h = tid / TC;
-#pragma unroll 4
-    for (int i = tid / TC; i < k * H; i += RG) {
-      while (h >= H) h -= H, ++j;
+  if (col < d)
+    for (int j = 0; j < js; ++j) {
       const int e = es[j];
-      if (e >= 0) {
+      if (e < 0) continue;
+      const T* const w2 = (const T*)c.w2 + (int64_t)e * H * d + col;
+#pragma unroll 4
+      for (int h = tid / TC; h < H; h += RG) {
         float f[V];
-        load_row<T, V>((const T*)c.w2 + ((int64_t)e * H + h) * d + col, f);
-        const float hv = hs[i];
+        load_row<T, V>(w2 + (int64_t)h * d, f);
+        const float hv = hs[j * H + h];
 #pragma unroll
         for (int q = 0; q < V; ++q) a[q] = fmaf(hv, f[q], a[q]);
       }
-      h += RG;
     }
-  }
   float sum = few_sum<V>(a, red);
-  const int at = blockIdx.x * TC * V + tid;
-  if (tid < TC * V && at < d) {
+  if (tid < TC * V) sums[tid] = sum;
+  cluster.sync();
+  if (rank == 0 && tid < TC * V && col0 + tid < d) {
+    for (int r = 1; r < ctas; ++r) sum += cluster.map_shared_rank(sums, r)[tid];
+    const int at = col0 + tid;
     if (c.last_bias) sum += DT<T>::to_f(((const T*)c.last_bias)[at]);
     if (c.add_residual) sum += DT<T>::to_f(((const T*)c.x)[t * d + at]);
     ((T*)c.out)[t * d + at] = DT<T>::from_f(sum);
   }
+  cluster.sync();                           // the others' sums are read until here
 }
 
 // -- host ----------------------------------------------------------------------------------------------------
@@ -357,26 +426,31 @@ int few_splits(int64_t P, int d, int H, int V) {
 }
 constexpr int MOST_SPLITS = 16;
 
+// Pairs of a thread in the sort: 4 up to 256 blocks of 1024 pairs, 16 beyond (fewer rows of counts for every block to add up;
+// past a million pairs they grow again).
 struct Sort {
-  int64_t chunk;
-  int blocks;
+  int per_thread, blocks, EP;
 };
-Sort sort_shape(int64_t P) {
-  if (P <= ONE_BLOCK_PAIRS) return {P, 1};
-  const int64_t chunk = (ceil_div64(P, CHUNK_BLOCKS) + NT - 1) / NT * NT;
-  return {chunk, (int)ceil_div64(P, chunk)};
+Sort sort_shape(int64_t P, int E) {
+  Sort s;
+  s.per_thread = P <= 256 * 4 * NT ? 4 : 16;
+  s.blocks = (int)ceil_div64(P, (int64_t)s.per_thread * NT);
+  s.EP = (E + 7) / 8 * 8;
+  return s;
 }
 
 struct Layout {                             // of the workspace, bytes
   size_t offsets, pairs, table, rows, total;
 };
-Layout layout_of(int64_t P, int d, int E, int dtype) {
+// tiles: the tensor-core kernel's rows
+Layout layout_of(int64_t P, int d, int E, bool tiles) {
+  const Sort s = sort_shape(P, E);
   Layout l;
   l.offsets = 0;
   l.pairs = up256((size_t)(E + 1) * 4);
   l.table = l.pairs + up256((size_t)P * 4);
-  l.rows = l.table + up256((size_t)sort_shape(P).blocks * E * 4);
-  l.total = l.rows + up256((size_t)P * d * (dtype == D2D_F32 ? 4 : 2));
+  l.rows = l.table + up256((size_t)s.blocks * s.EP * 2);
+  l.total = l.rows + up256((size_t)P * d * (tiles ? 2 : 4));
   return l;
 }
 
@@ -384,14 +458,19 @@ template <typename T, int V, bool GLU>
 int few(const WeightedCall& c, float* part, cudaStream_t s) {
   const int64_t P = c.N * c.k;
   const int splits = few_splits(P, c.d, c.H, V), cols = few_threads<V> * V;
-  const size_t smem = ((size_t)c.k * c.H + c.k) * sizeof(float);
+  // CTAs of a cluster: a slot each, unless there are blocks enough
+  const int64_t blocks = (int64_t)ceil_div(c.d, cols) * c.N;
+  int ctas = 1;
+  while (ctas < 8 && 2 * ctas <= c.k && 2 * ctas * blocks <= 1024) ctas *= 2;
+  const int share = ceil_div(c.k, ctas);
+  const size_t smem = ((size_t)share * c.H + share) * sizeof(float);
   int rc = device_launch_facts((const void*)few_out_kernel<T, V, GLU>, smem, nullptr);
   if (rc != D2D_OK) return rc;
   rc = launch_pdl(few_hidden_kernel<T, V, GLU>, dim3((unsigned)(ceil_div(c.H, cols) * splits), (unsigned)P), dim3(NT),
                   0, s, c, splits, part);
   if (rc != D2D_OK) return rc;
-  return launch_pdl(few_out_kernel<T, V, GLU>, dim3((unsigned)ceil_div(c.d, cols), (unsigned)c.N), dim3(NT), smem, s,
-                    c, splits, (const float*)part);
+  return launch_pdl_cluster(ctas, few_out_kernel<T, V, GLU>, dim3((unsigned)(ceil_div(c.d, cols) * ctas), (unsigned)c.N),
+                            dim3(NT), smem, s, c, splits, share, (const float*)part);
 }
 template <typename T>
 int few_t(const WeightedCall& c, float* part, cudaStream_t s) {
@@ -401,23 +480,26 @@ int few_t(const WeightedCall& c, float* part, cudaStream_t s) {
   return vec ? few<T, V, false>(c, part, s) : few<T, 1, false>(c, part, s);
 }
 
+template <typename T, int V, bool CODED>
+int combine_v(const WeightedCall& c, const void* y, cudaStream_t s) {
+  const int nv = c.d / V, tokens = std::max(1, 2 * NT / nv);
+  return launch_pdl(combine_kernel<T, V, CODED>, dim3((unsigned)ceil_div64(c.N, tokens)), dim3(NT), 0, s, y, c.experts,
+                    c.weights, (const T*)c.last_bias, c.add_residual ? (const T*)c.x : nullptr, (T*)c.out, c.N, c.d, c.E,
+                    c.k, tokens);
+}
 template <typename T>
-int combine_t(const WeightedCall& c, const void* y, int sms, cudaStream_t s) {
+int combine_t(const WeightedCall& c, const void* y, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = c.d % V == 0 && al16(c.x) && al16(c.out) && al16(c.last_bias);
-  const int64_t need = ceil_div64(c.N, NT / 32), most = (int64_t)sms * 8;
-  const dim3 grid((unsigned)(need < most ? need : most));
-  const auto k = vec ? combine_kernel<T, V> : combine_kernel<T, 1>;
-  return launch_pdl(k, grid, dim3(NT), 0, s, (const T*)y, c.experts, c.weights, (const T*)c.last_bias,
-                    c.add_residual ? (const T*)c.x : nullptr, (T*)c.out, c.N, c.d, c.E, c.k);
+  return vec ? combine_v<T, V, false>(c, y, s) : combine_v<T, 1, false>(c, y, s);
 }
 
 }  // namespace
 
-size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, int dtype) {
+size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, bool tiles) {
   const int64_t P = N * k;
   if (takes_few(P, d, H, k)) return up256((size_t)MOST_SPLITS * P * (glu ? 2 : 1) * H * sizeof(float));
-  return layout_of(P, d, E, dtype).total;
+  return layout_of(P, d, E, tiles).total;
 }
 
 bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, bool tiles) {
@@ -432,28 +514,32 @@ int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s) {
   const int64_t P = c.N * c.k;
   if (takes_few(P, c.d, c.H, c.k))
     return c.dtype == D2D_F32 ? few_t<float>(c, (float*)ws, s) : few_t<bf16>(c, (float*)ws, s);
-  const Layout l = layout_of(P, c.d, c.E, c.dtype);
+  const Layout l = layout_of(P, c.d, c.E, c.packed != nullptr);
   uint8_t* const base = (uint8_t*)ws;
   int32_t* const offsets = (int32_t*)(base + l.offsets);
   int32_t* const pairs = (int32_t*)(base + l.pairs);
-  int32_t* const table = (int32_t*)(base + l.table);
+  uint16_t* const table = (uint16_t*)(base + l.table);
   void* const rows = base + l.rows;
-  const Sort st = sort_shape(P);
-  const int threads = st.blocks == 1 ? 1024 : NT;
+  const Sort st = sort_shape(P, c.E);
+  const dim3 grid((unsigned)st.blocks);
   if (st.blocks > 1) {
-    rc = launch_pdl(pairs_count_kernel, dim3((unsigned)st.blocks), dim3(NT), 0, s, c.experts, P, c.E, st.chunk, table);
+    rc = launch_pdl(st.per_thread == 4 ? pairs_count_kernel<4> : pairs_count_kernel<16>, grid, dim3(NT), 0, s, c.experts,
+                    P, c.E, st.EP, table);
     if (rc != D2D_OK) return rc;
   }
-  const size_t smem = ((size_t)(threads / 32) * c.E + 3 * (size_t)c.E + 1) * sizeof(int);
-  rc = launch_pdl(pairs_scatter_kernel, dim3((unsigned)st.blocks), dim3((unsigned)threads), smem, s, c.experts, P, c.E,
-                  st.chunk, st.blocks > 1 ? (const int32_t*)table : nullptr, pairs, offsets, c.dev_status);
+  rc = launch_pdl(st.per_thread == 4 ? pairs_scatter_kernel<4> : pairs_scatter_kernel<16>, grid, dim3(NT), 0, s,
+                  c.experts, P, c.E, st.EP, st.blocks > 1 ? (const uint16_t*)table : nullptr, pairs, offsets,
+                  c.dev_status);
   if (rc != D2D_OK) return rc;
-  rc = c.packed ? launch_experts_umma_pairs(c.x, pairs, offsets, c.packed, rows, c.N, c.d, c.E, c.H, c.k,
-                                            c.w_up != nullptr, c.act, c.dev_status, s)
-                : launch_experts_simt_pairs(c.x, pairs, offsets, c.w1, c.b1, c.w_up, c.w2, rows, c.N, c.d, c.E, c.H,
-                                            c.k, c.act, c.dtype, c.dev_status, s);
+  if (c.packed) {
+    rc = launch_experts_umma_pairs(c.x, pairs, offsets, c.packed, rows, c.N, c.d, c.E, c.H, c.k, c.w_up != nullptr,
+                                   c.act, c.dev_status, s);
+    return rc != D2D_OK ? rc : combine_v<bf16, 8, true>(c, rows, s);
+  }
+  rc = launch_experts_simt_pairs(c.x, pairs, offsets, c.w1, c.b1, c.w_up, c.w2, rows, c.N, c.d, c.E, c.H, c.k, c.act,
+                                 c.dtype, c.dev_status, s);
   if (rc != D2D_OK) return rc;
-  return c.dtype == D2D_F32 ? combine_t<float>(c, rows, sms, s) : combine_t<bf16>(c, rows, sms, s);
+  return c.dtype == D2D_F32 ? combine_t<float>(c, rows, s) : combine_t<bf16>(c, rows, s);
 }
 
 }  // namespace d2d

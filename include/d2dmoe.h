@@ -273,13 +273,12 @@ int d2d_route_backward(const void* logits, const int32_t* experts, const float* 
  *   y[t,j,:] = act(x[t,:] W1[e] + b1[e]) (* x[t,:] W_up[e]) W2[e],  e = experts[t,j]
  * for experts [N, k] (i32; -1: no such slot; the same expert may stand in several) and weights [N, k] (fp32).  A
  * token's sum is held in fp32, taken in the order of its slots and rounded once.  The hidden values are
- * rounded once (bf16 tensor-core path) or not at all, y to T, except in calls of few pairs, where nothing is
- * rounded before the end.  The same call gives the same bits.  An expert outside -1..E-1 is skipped and reported
+ * rounded once and y to 2^-14 of the largest of eight columns (bf16 tensor-core path), neither elsewhere.  The same call gives the same bits.  An expert outside -1..E-1 is skipped and reported
  * (D2D_ERR_INDEX_RANGE in *dev_status).  k <= min(32, E), E <= 256, N k < 2^31 - 1.  experts_packed_opt as for
- * d2d_experts_ffn; shapes and buffers that the tensor-core kernels do not take go to the general-shape ones.
- * ws: d2d_experts_weighted_workspace_bytes, 256-byte aligned.  (Upstream's dense form multiplies every
+ * d2d_experts_ffn.  x and out start on 16-byte boundaries, with packed weights last_bias too.
+ * ws: d2d_experts_weighted_workspace_bytes (packed: whether experts_packed_opt is given), 256-byte aligned.  (Upstream's dense form multiplies every
  * expert's output by its routing entry: architectures/moe/moe_layers.py:91-101.) */
-int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int dtype,
+int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, int glu, int packed, int dtype,
                                          size_t* bytes /* host */);
 int d2d_experts_weighted(const void* x, const int32_t* experts, const float* weights, const void* w1,
                          const void* b1_opt, const void* w_up_opt, const void* w2, const void* experts_packed_opt,
