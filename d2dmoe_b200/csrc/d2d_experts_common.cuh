@@ -118,56 +118,88 @@ __device__ __forceinline__ void add_row(void* p, int t, uint4 v) {
       : "memory");
 }
 
-// Eight floats in 16 bytes: 15-bit integers in units of a common power of two, 2^-13 of the one above the largest.  A bf16 row
-// would be as large and 2^-9 off at every element; this is 2^-14 off of the largest of eight.  The exponent (that of the
-// largest, as floats have it) lies in the lowest bits of the eight halves.  Exponent 255, where one is not
-// finite: the halves are bf16 without their lowest bit.
-__device__ __forceinline__ uint4 encode8(const float (&f)[8]) {
-  float m = fabsf(f[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(f[i])));
-  uint32_t ex = __float_as_uint(m) >> 23;
-  uint32_t w[4];
-  if (ex == 255u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]) & 0xfffefffeu;
-  } else {
-    ex = max(ex, 13u);
-    const float s = __uint_as_float((266u - ex) << 23);      // 2^(139 - ex): |f s| < 2^13
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = __float_as_uint(fmaf(f[2 * i], s, 12582912.f)),
-                     b = __float_as_uint(fmaf(f[2 * i + 1], s, 12582912.f));     // 1.5 2^23: the integer is below
-      w[i] = (__byte_perm(a, b, 0x5410) << 1) & 0xfffefffeu;
-    }
-  }
-  const uint32_t z = ex | ex << 15;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] |= (z >> (2 * i)) & 0x00010001u;
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// Eight floats in 16 bytes: 15-bit integers in units of 2^(ex - 140) / (1 - 2^-14), where 2^(ex - 127) is the largest's power
+// of two: off by half a unit, 2^-14 of the largest of eight (bf16, as many bytes, would be by 2^-8 of each).  The
+// last factor keeps them below 2^14; they are held with 2^14 added.  The exponent lies in the upper bits of the
+// eight halves.  Exponent 255, where one is not finite: the halves are the upper 15 bits of bf16.
+struct Eight {
+  uint32_t f[8];           // bits of floats
+};
+__device__ __forceinline__ uint32_t exponent8(const Eight& v) {
+  float m;
+  asm("{\n\t.reg .f32 a, b, c, d, e, f, g, h;\n\t"
+      "abs.f32 a, %1;\n\tabs.f32 b, %2;\n\tabs.f32 c, %3;\n\tabs.f32 d, %4;\n\t"
+      "abs.f32 e, %5;\n\tabs.f32 f, %6;\n\tabs.f32 g, %7;\n\tabs.f32 h, %8;\n\t"
+      "max.NaN.f32 a, a, b, c;\n\tmax.NaN.f32 d, d, e, f;\n\tmax.NaN.f32 g, g, h;\n\tmax.NaN.f32 %0, a, d, g;\n\t}"
+      : "=f"(m)
+      : "f"(__uint_as_float(v.f[0])), "f"(__uint_as_float(v.f[1])), "f"(__uint_as_float(v.f[2])),
+        "f"(__uint_as_float(v.f[3])), "f"(__uint_as_float(v.f[4])), "f"(__uint_as_float(v.f[5])),
+        "f"(__uint_as_float(v.f[6])), "f"(__uint_as_float(v.f[7])));
+  return __float_as_uint(m) >> 23;
 }
-// sum += wt * the eight
-__device__ __forceinline__ void add_decoded8(uint4 v, float wt, float (&sum)[8]) {
+__device__ __forceinline__ uint4 with_exponent(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t ex) {
+  const uint32_t z = ex | ex << 15, m = 0x80008000u;       // bit 2 i to 15, bit 2 i + 1 to 31
+  return make_uint4((a & ~m) | (z << 15 & m), (b & ~m) | (z << 13 & m), (c & ~m) | (z << 11 & m),
+                    (d & ~m) | (z << 9 & m));
+}
+// ex: exponent8(v), below 255
+__device__ __forceinline__ uint4 encode8(const Eight& v, uint32_t ex) {
+  ex = max(ex, 14u);
+  const float s = __uint_as_float(((266u - ex) << 23) + 0x7ffe00u);      // 2^(140 - ex) (1 - 2^-14): |f s| <= 2^14 - 1
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {                              // 1.5 2^23 + 2^14: the integer is in the lower half
+    uint32_t lo, hi;
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(v.f[2 * i]), "r"(v.f[2 * i + 1]), "f"(s), "f"(12582912.f + 16384.f));
+    w[i] = __byte_perm(lo, hi, 0x5410);
+  }
+  return with_exponent(w[0], w[1], w[2], w[3], ex);
+}
+// at least one is not finite
+static __device__ __noinline__ uint4 encode8_special(const Eight v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = pack_bf16x2(__uint_as_float(v.f[2 * i]), __uint_as_float(v.f[2 * i + 1]));
+    w[i] = w[i] >> 1 & 0x7fff7fffu;
+  }
+  return with_exponent(w[0], w[1], w[2], w[3], 255u);
+}
+__device__ __forceinline__ uint32_t exponent_of(uint4 v) {
+  const uint32_t y = (v.x >> 15 & 0x00010001u) | (v.y >> 13 & 0x00040004u) | (v.z >> 11 & 0x00100010u) |
+                     (v.w >> 9 & 0x00400040u);
+  return (y | y >> 15) & 255u;
+}
+// sum += wt * the eight (pairs of floats); ex: exponent_of(v); wt: with UNIT8 multiplied in
+constexpr float UNIT8 = 1.00006103888177f;                   // 1 / (1 - 2^-14)
+__device__ __forceinline__ void add_decoded8(uint4 v, uint32_t ex, float wt, unsigned long long (&sum)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  uint32_t ex = 0u;
+  const float s = wt * __uint_as_float((ex - 13u) << 23);    // 2^(ex - 140)
+  unsigned long long s2, c2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(-(8388608.f + 16384.f)));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t t = w[i] & 0x00010001u;
-    ex |= ((t | t >> 15) & 3u) << (2 * i);
+    const uint32_t u = w[i] & 0x7fff7fffu;
+    unsigned long long x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "r"(__byte_perm(u, 0x4b00u, 0x5410)), "r"(__byte_perm(u, 0x4b00u, 0x5432)));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(c2));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum[i]) : "l"(x), "l"(s2));
   }
-  if (ex == 255u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[2 * i] = fmaf(wt, __uint_as_float(w[i] << 16 & 0xfffe0000u), sum[2 * i]);
-      sum[2 * i + 1] = fmaf(wt, __uint_as_float(w[i] & 0xfffe0000u), sum[2 * i + 1]);
-    }
-    return;
-  }
-  const float s = __uint_as_float((ex - 12u) << 23);         // 2^(ex - 139)
+}
+__device__ __forceinline__ void add_special8(uint4 v, float wt, unsigned long long (&sum)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    sum[2 * i] = fmaf(wt, (float)((int32_t)(w[i] << 16) >> 17) * s, sum[2 * i]);
-    sum[2 * i + 1] = fmaf(wt, (float)((int32_t)w[i] >> 17) * s, sum[2 * i + 1]);
+    float lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(sum[i]));
+    lo = fmaf(wt, __uint_as_float((w[i] & 0x7fffu) << 17), lo);
+    hi = fmaf(wt, __uint_as_float((w[i] >> 16 & 0x7fffu) << 17), hi);
+    asm("mov.b64 %0, {%1, %2};" : "=l"(sum[i]) : "f"(lo), "f"(hi));
   }
 }
 

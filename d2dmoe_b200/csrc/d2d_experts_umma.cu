@@ -968,15 +968,30 @@ __device__ void role_drain_pairs(const Params& p, Ctl* c, uint32_t tmem, int j, 
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint4 w[2][2];                   // [row rl + 8 i][block of 32 columns]
+        Eight f[2][2];
+        uint32_t ex[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float f[8];
 #pragma unroll
-            for (int h = 0; h < 8; ++h) f[h] = __uint_as_float(v[16 * k + 4 * (h >> 1) + 2 * i + (h & 1)]);
-            w[i][k] = encode8(f);
+            for (int h = 0; h < 8; ++h) f[i][k].f[h] = v[16 * k + 4 * (h >> 1) + 2 * i + (h & 1)];
+            ex[i][k] = exponent8(f[i][k]);
           }
+        // (one branch for all four: they are worked on side by side)
+        if (max(max(ex[0][0], ex[0][1]), max(ex[1][0], ex[1][1])) < 255u) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) w[i][k] = encode8(f[i][k], ex[i][k]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              w[i][k] = ex[i][k] < 255u ? encode8(f[i][k], ex[i][k]) : encode8_special(f[i][k]);
+        }
+        __syncwarp();
         if (half == 0) tmem_ld_frag64(acc + (16u << 16), v);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

@@ -135,7 +135,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 
 // c: room for E numbers of this warp
 template <typename T>
-__device__ __noinline__ void route_exact(const RouteArgs& a, int64_t t, double* c, int lane) {
+__device__ __noinline__ void route_exact(const RouteArgs a, int64_t t, double* c, int lane) {
   const T* row = reinterpret_cast<const T*>(a.logits) + t * a.E;
   const double none = -INFINITY;
   const int E = a.E;

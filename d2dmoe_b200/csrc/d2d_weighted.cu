@@ -182,6 +182,15 @@ __device__ __forceinline__ void load_row(const T* p, float* f) {
     }
   }
 }
+template <int V>
+__device__ __forceinline__ void load_plain(const float* p, float* f) {
+  if constexpr (V == 1) f[0] = *p;
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    const float4 a = *(reinterpret_cast<const float4*>(p) + i);
+    f[4 * i] = a.x, f[4 * i + 1] = a.y, f[4 * i + 2] = a.z, f[4 * i + 3] = a.w;
+  }
+}
 template <typename T, int V>
 __device__ __forceinline__ void store_row(T* p, const float* f) {
   if constexpr (V == 1) {
@@ -194,61 +203,70 @@ __device__ __forceinline__ void store_row(T* p, const float* f) {
   }
 }
 
-// y: [N k, d] fp32 or (CODED) in pieces of encode8.  A thread has V columns of a token; a block takes a few tokens.
-template <typename T, int V, bool CODED>
+// The sum's weights of four slots: zero, and no row, where there is no expert.  fours: 16-byte loads
+struct Slots {
+  float w[4];
+  bool there[4];
+};
+__device__ __forceinline__ Slots load_slots(const int32_t* e, const float* w, int left, int E, bool fours) {
+  int4 e4;
+  float4 w4;
+  if (fours) {
+    e4 = *reinterpret_cast<const int4*>(e);
+    w4 = *reinterpret_cast<const float4*>(w);
+  } else {
+    e4 = make_int4(e[0], left > 1 ? e[1] : -1, left > 2 ? e[2] : -1, left > 3 ? e[3] : -1);
+    w4 = make_float4(w[0], left > 1 ? w[1] : 0.f, left > 2 ? w[2] : 0.f, left > 3 ? w[3] : 0.f);
+  }
+  Slots s;
+  const int ee[4] = {e4.x, e4.y, e4.z, e4.w};
+  const float ww[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    s.there[u] = (unsigned)ee[u] < (unsigned)E;
+    s.w[u] = s.there[u] ? ww[u] : 0.f;
+  }
+  return s;
+}
+__device__ __forceinline__ bool by_fours(const int32_t* e, const float* w, int k) {
+  return k % 4 == 0 && ((reinterpret_cast<uintptr_t>(e) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
+}
+
+// y: [N k, d] fp32.  A thread has V columns of a token; a block takes a few tokens.  per_row: ceil(2^32 / (d / V))
+template <typename T, int V>
 __global__ void __launch_bounds__(NT)
-combine_kernel(const void* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
+combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
                const T* __restrict__ last_bias, const T* __restrict__ x, T* __restrict__ out, int64_t N, int d,
-               int E, int k, int tokens) {
+               int E, int k, int tokens, uint32_t per_row) {
   grid_launch_dependents();
   grid_dependency_wait();
   fresh(y, experts, weights, last_bias, x);
   const int nv = d / V;
   const int64_t t0 = (int64_t)blockIdx.x * tokens;
   const int items = (int)min((int64_t)tokens, N - t0) * nv;
+  const bool fours = by_fours(experts, weights, k);
   for (int i = threadIdx.x; i < items; i += NT) {
-    const int dt = i / nv, c = (i - dt * nv) * V;
+    const int dt = nv == 1 ? i : (int)__umulhi((uint32_t)i, per_row), c = (i - dt * nv) * V;
     const int64_t t = t0 + dt;
+    const float* row = y + t * k * d + c;
     float sum[V], f[V];
 #pragma unroll
     for (int q = 0; q < V; ++q) sum[q] = 0.f;
     // (four rows' loads at a time, asked for before the first is used)
-    for (int j0 = 0; j0 < k; j0 += 4) {
-      uint4 raw[4];
-      float4 lo[4], hi[4];
-      float wt[4];
+    for (int j = 0; j < k; j += 4) {
+      const Slots s = load_slots(experts + t * k + j, weights + t * k + j, k - j, E, fours);
+      float v[4][V];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int j = j0 + u;
-        const int e = j < k ? __ldg(experts + t * k + j) : -1;
-        wt[u] = 0.f;
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if ((unsigned)e < (unsigned)E) {
-          wt[u] = __ldg(weights + t * k + j);
-          const int64_t at = (t * k + j) * d + c;
-          if constexpr (CODED) {
-            raw[u] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(y) + at));
-          } else {
-            const float* p = reinterpret_cast<const float*>(y) + at;
-            if constexpr (V == 1) lo[u].x = __ldg(p);
-            if constexpr (V >= 4) lo[u] = __ldg(reinterpret_cast<const float4*>(p));
-            if constexpr (V == 8) hi[u] = __ldg(reinterpret_cast<const float4*>(p) + 1);
-          }
-        } else {
-          wt[u] = 0.f;
-        }
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[u][q] = 0.f;
+        if (s.there[u]) load_plain<V>(row, v[u]);
+        row += d;
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if constexpr (CODED) {
-          if (j0 + u < k) umma::add_decoded8(raw[u], wt[u], sum);      // (no expert: zeros of weight zero)
-        } else {
-          const float v[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int q = 0; q < V; ++q) sum[q] = fmaf(wt[u], v[q], sum[q]);
-        }
-      }
+        for (int q = 0; q < V; ++q) sum[q] = fmaf(s.w[u], v[u][q], sum[q]);
     }
     if (last_bias) {
       load_row<T, V>(last_bias + c, f);
@@ -262,6 +280,159 @@ combine_kernel(const void* __restrict__ y, const int32_t* __restrict__ experts, 
     }
     store_row<T, V>(out + t * d + c, sum);
   }
+}
+
+// y: [N k, d] in pieces of encode8, which bound this kernel: 310 of 464 MB at 50432 tokens x 4 x 768, 78 us.  A thread has two
+// pieces of a token, half a row apart, and goes through the tokens with the grid; the four rows (and x) of its next turn
+// travel by cp.async into slots of its own.  (One piece a thread: 94 us, half of it instructions; loads into registers: 101.
+// Blocks of 128 threads and 3 or 4 turns ahead, so fewer warps: 84, 104.)
+constexpr int COMBINE_NT = 256, COMBINE_STAGES = 2, COMBINE_ROWS = 5;
+constexpr size_t COMBINE_SMEM = (size_t)COMBINE_STAGES * COMBINE_ROWS * 2 * COMBINE_NT * 16;
+constexpr int COMBINE_BLOCKS = (int)(220 * 1024 / COMBINE_SMEM);       // of an SM
+__global__ void __launch_bounds__(COMBINE_NT, COMBINE_BLOCKS)
+combine_coded_kernel(const uint16_t* __restrict__ y, const int32_t* __restrict__ experts,
+                     const float* __restrict__ weights, const bf16* __restrict__ last_bias, const bf16* __restrict__ x,
+                     bf16* __restrict__ out, int64_t N, int d, int E, int k) {
+  extern __shared__ __align__(16) uint4 ring[];      // [stage][row][piece][thread]
+  grid_launch_dependents();
+  grid_dependency_wait();
+  fresh(y, experts, weights, last_bias, x);
+  constexpr int NT = COMBINE_NT, ROW = 2 * NT;                // uint4 of a row of a stage
+  const int nv = d / 16, groups = (k + 3) / 4;
+  const bool fours = by_fours(experts, weights, k);
+  const int64_t stride = (int64_t)gridDim.x * NT;
+  const int dt = (int)(stride / nv), dc = (int)(stride - (int64_t)dt * nv);
+  const int64_t first = (int64_t)blockIdx.x * NT + threadIdx.x, t0 = first / nv;
+  // A turn: four slots (group g) of token t, columns 16 c ..; what moves with it are pointers.
+  struct At {
+    int64_t t;
+    int c, g;
+  };
+  At now = {t0, (int)(first - t0 * nv), 0}, ask = now;
+  const uint16_t* ask_y = y + t0 * k * d + 8 * ask.c;
+  const bf16* ask_x = x ? x + t0 * d + 8 * ask.c : nullptr;
+  bf16* to = out + t0 * d + 8 * now.c;
+  const int32_t* e = experts + t0 * k;
+  const float* w = weights + t0 * k;
+  const int64_t dy = (int64_t)dt * k * d + 8 * dc - (int64_t)(groups - 1) * 4 * d;
+  const int64_t wrap_y = (int64_t)k * d - d / 2, dx = (int64_t)dt * d + 8 * dc;
+  const int ds = dt * k - (groups - 1) * 4;
+  uint32_t fill = (uint32_t)__cvta_generic_to_shared(ring + threadIdx.x);
+  const uint32_t end = fill + COMBINE_STAGES * COMBINE_ROWS * ROW * 16;
+  auto fetch = [&]() {
+    if (ask.t < N) {
+      const int left = k - 4 * ask.g;
+      const uint16_t* row = ask_y;
+#pragma unroll
+      for (int u = 0; u < 4; ++u, row += d)
+        if (u < left)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0 + %2], [%3], 16;" ::"r"(
+                           fill + u * ROW * 16),
+                       "l"(row), "n"(NT * 16), "l"(row + d / 2)
+                       : "memory");
+      if (x && left <= 4)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n\tcp.async.cg.shared.global [%0 + %2], [%3], 16;" ::"r"(
+                         fill + 4 * ROW * 16),
+                     "l"(ask_x), "n"(NT * 16), "l"(ask_x + d / 2)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fill += COMBINE_ROWS * ROW * 16;
+    if (fill >= end) fill -= COMBINE_STAGES * COMBINE_ROWS * ROW * 16;
+    if (++ask.g < groups) {
+      ask_y += 4 * (int64_t)d;
+      return;
+    }
+    ask.g = 0;
+    ask.t += dt;
+    ask.c += dc;
+    ask_y += dy;
+    ask_x += dx;
+    if (ask.c >= nv) ask.c -= nv, ++ask.t, ask_y += wrap_y, ask_x += d / 2;
+  };
+#pragma unroll
+  for (int i = 0; i < COMBINE_STAGES - 1; ++i) fetch();
+  Slots s = {};
+  if (now.t < N) s = load_slots(e, w, k, E, fours);
+  const uint4* at = ring + threadIdx.x;
+  unsigned long long sum[2][4];
+  while (now.t < N) {
+    At next = now;
+    if (++next.g < groups) {
+      e += 4, w += 4;
+    } else {
+      next.g = 0;
+      next.t += dt;
+      next.c += dc;
+      e += ds, w += ds;
+      if (next.c >= nv) next.c -= nv, ++next.t, e += k, w += k;
+    }
+    Slots s1 = s;                            // the next turn's, asked for now
+    if (next.t < N) s1 = load_slots(e, w, k - 4 * next.g, E, fours);
+    asm volatile("cp.async.wait_group %0;" ::"n"(COMBINE_STAGES - 2) : "memory");
+    uint4 raw[4][2], xr[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) raw[u][p] = at[u * ROW + p * NT];
+      xr[p] = at[4 * ROW + p * NT];
+    }
+    at += COMBINE_ROWS * ROW;
+    if (at >= ring + COMBINE_STAGES * COMBINE_ROWS * ROW) at -= COMBINE_STAGES * COMBINE_ROWS * ROW;
+    fetch();
+    uint32_t ex[4][2], most = 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {          // (no expert, no slot: whatever lay there, as finite numbers, times zero)
+        ex[u][p] = s.there[u] ? umma::exponent_of(raw[u][p]) : 14u;
+        most = max(most, ex[u][p]);
+      }
+    if (now.g == 0)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[0][i] = sum[1][i] = 0;
+    if (most < 255u) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) umma::add_decoded8(raw[u][p], ex[u][p], s.w[u] * umma::UNIT8, sum[p]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          if (ex[u][p] < 255u) umma::add_decoded8(raw[u][p], ex[u][p], s.w[u] * umma::UNIT8, sum[p]);
+          else umma::add_special8(raw[u][p], s.w[u], sum[p]);
+        }
+    }
+    if (next.g == 0) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float f[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "l"(sum[p][i]));
+        if (last_bias) {
+          load_row<bf16, 8>(last_bias + 8 * now.c + p * (d / 2), b);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) f[q] += b[q];
+        }
+        if (x) {
+          const uint32_t v[4] = {xr[p].x, xr[p].y, xr[p].z, xr[p].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] += __uint_as_float(v[i] << 16);
+            f[2 * i + 1] += __uint_as_float(v[i] & 0xffff0000u);
+          }
+        }
+        store_row<bf16, 8>(to + p * (d / 2), f);
+      }
+      to += dx;
+      if (next.t > now.t + dt) to += d / 2;
+    }
+    now = next;
+    s = s1;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // -- few pairs ---------------------------------------------------------------------------------------------
@@ -480,18 +651,27 @@ int few_t(const WeightedCall& c, float* part, cudaStream_t s) {
   return vec ? few<T, V, false>(c, part, s) : few<T, 1, false>(c, part, s);
 }
 
-template <typename T, int V, bool CODED>
+template <typename T, int V>
 int combine_v(const WeightedCall& c, const void* y, cudaStream_t s) {
   const int nv = c.d / V, tokens = std::max(1, 2 * NT / nv);
-  return launch_pdl(combine_kernel<T, V, CODED>, dim3((unsigned)ceil_div64(c.N, tokens)), dim3(NT), 0, s, y, c.experts,
-                    c.weights, (const T*)c.last_bias, c.add_residual ? (const T*)c.x : nullptr, (T*)c.out, c.N, c.d, c.E,
-                    c.k, tokens);
+  return launch_pdl(combine_kernel<T, V>, dim3((unsigned)ceil_div64(c.N, tokens)), dim3(NT), 0, s, (const float*)y,
+                    c.experts, c.weights, (const T*)c.last_bias, c.add_residual ? (const T*)c.x : nullptr, (T*)c.out, c.N,
+                    c.d, c.E, c.k, tokens, (uint32_t)((0x100000000ULL + nv - 1) / nv));
 }
 template <typename T>
 int combine_t(const WeightedCall& c, const void* y, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = c.d % V == 0 && al16(c.x) && al16(c.out) && al16(c.last_bias);
-  return vec ? combine_v<T, V, false>(c, y, s) : combine_v<T, 1, false>(c, y, s);
+  return vec ? combine_v<T, V>(c, y, s) : combine_v<T, 1>(c, y, s);
+}
+int combine_coded(const WeightedCall& c, const void* y, int sms, cudaStream_t s) {
+  const int rc = device_launch_facts((const void*)combine_coded_kernel, COMBINE_SMEM, nullptr);
+  if (rc != D2D_OK) return rc;
+  const int64_t need = ceil_div64(c.N * (c.d / 16), COMBINE_NT);
+  return launch_pdl(combine_coded_kernel, dim3((unsigned)std::min<int64_t>(need, COMBINE_BLOCKS * sms)), dim3(COMBINE_NT),
+                    COMBINE_SMEM, s,
+                    (const uint16_t*)y, c.experts, c.weights, (const bf16*)c.last_bias,
+                    c.add_residual ? (const bf16*)c.x : nullptr, (bf16*)c.out, c.N, c.d, c.E, c.k);
 }
 
 }  // namespace
@@ -534,7 +714,7 @@ int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s) {
   if (c.packed) {
     rc = launch_experts_umma_pairs(c.x, pairs, offsets, c.packed, rows, c.N, c.d, c.E, c.H, c.k, c.w_up != nullptr,
                                    c.act, c.dev_status, s);
-    return rc != D2D_OK ? rc : combine_v<bf16, 8, true>(c, rows, s);
+    return rc != D2D_OK ? rc : combine_coded(c, rows, sms, s);
   }
   rc = launch_experts_simt_pairs(c.x, pairs, offsets, c.w1, c.b1, c.w_up, c.w2, rows, c.N, c.d, c.E, c.H, c.k, c.act,
                                  c.dtype, c.dev_status, s);

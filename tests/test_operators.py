@@ -546,6 +546,40 @@ def test_weighted_experts_odd_choices(N, dtype):
 
 
 @pytest.mark.gpu
+def test_weighted_experts_sizes_and_infinities():
+    """Outputs of very different sizes beside each other, tiny, huge and zero rows; infinities and NaN stay what they are
+    in their own columns."""
+    import d2dmoe_b200 as D
+    x, e, w, w1, b1, w2, up, lb = experts_case(300, 128, 12, 32, 3, "bf16", False, True, seed=4)
+    e[:, 0], e[:, 1], e[:, 2] = 0, 1, 2
+    w2[0] *= torch.logspace(-30, 30, 128, device="cuda").to(w2.dtype)
+    w2[1] *= 1e-36
+    w2[2] = 0.0
+    packed = D.ops.prepack_experts(w1, b1, w2)
+    for k in (3, 1):
+        got = D.ops.experts_weighted(x, e[:, :k].contiguous(), w[:, :k].contiguous(), w1, b1, w2, "relu", packed=packed)
+        want, tol = experts_reference(x, e[:, :k], w[:, :k], w1, b1, w2, "relu")
+        within(got, want, tol + 2e-38, "sizes")
+    w2[3] = w2[4]
+    w2[3, :, 5] = 3e38                                   # one column overflows
+    packed = D.ops.prepack_experts(w1, b1, w2)
+    e[:, 0], e[:, 1] = 3, 4
+    x.abs_()
+    w1[3].abs_().mul_(30)                                # sums of 32 terms of about 3e38 times 10
+    packed = D.ops.prepack_experts(w1, b1, w2)
+    got = D.ops.experts_weighted(x, e, w, w1, b1, w2, "relu", packed=packed)
+    want, tol = experts_reference(x, e, w, w1, b1, w2, "relu")
+    assert torch.isinf(got[:, 5]).all()
+    keep = torch.arange(128, device="cuda") != 5
+    # (beside it the eight columns are bf16 without their lowest bit: 2^-7)
+    within(got[:, keep], want[:, keep], tol[:, keep] + 2.0 ** -7 * want[:, keep].abs().amax(), "beside an infinity")
+    assert torch.isfinite(got[:, keep]).all()
+    x[7, 3] = math.nan
+    got2 = D.ops.experts_weighted(x, e, w, w1, b1, w2, "gelu", packed=packed)
+    assert torch.isnan(got2[7]).all() and torch.isfinite(got2[8:, keep]).all()
+
+
+@pytest.mark.gpu
 def test_weighted_experts_strided_and_misaligned():
     import d2dmoe_b200 as D
     x, e, w, w1, b1, w2, up, lb = experts_case(200, 128, 12, 32, 4, "bf16", False, True, seed=2)
