@@ -187,7 +187,7 @@ int d2d_experts_weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, 
                                          size_t* bytes) {
   if (!bytes || N < 0 || d < 1 || E < 1 || H < 1 || k < 1 || k > E) return D2D_ERR_BAD_ARG;
   if (!dtype_ok(dtype)) return D2D_ERR_UNSUPPORTED;
-  *bytes = weighted_workspace_bytes(N, d, E, H, k, glu != 0,
+  *bytes = weighted_workspace_bytes(N, d, E, H, k, glu != 0, dtype,
                                     packed && umma_experts_supported(d, E, H, glu != 0, dtype));
   return D2D_OK;
 }
@@ -205,10 +205,10 @@ int d2d_experts_weighted(const void* x, const int32_t* experts, const float* wei
   if (!aligned(x, 16) || !aligned(out, 16) || !aligned(experts, 4) || !aligned(weights, 4) ||
       (tiles && (!aligned(experts_packed_opt, 1024) || !aligned(last_bias_opt, 16))))
     return D2D_ERR_BAD_ARG;
-  if (!weighted_supported(N, d, E, H, k, glu, tiles)) return D2D_ERR_UNSUPPORTED;
+  if (!weighted_supported(N, d, E, H, k, glu, dtype, tiles)) return D2D_ERR_UNSUPPORTED;
   if (N == 0) return D2D_OK;
   if (!ws || !aligned(ws, 256)) return D2D_ERR_BAD_ARG;
-  if (ws_bytes < weighted_workspace_bytes(N, d, E, H, k, glu, tiles)) return D2D_ERR_WORKSPACE;
+  if (ws_bytes < weighted_workspace_bytes(N, d, E, H, k, glu, dtype, tiles)) return D2D_ERR_WORKSPACE;
   const WeightedCall c = {x,       w1,  b1_opt, w_up_opt, w2, tiles ? experts_packed_opt : nullptr, last_bias_opt,
                           experts, weights, out, N, d, E, H, k, act, dtype, add_residual, dev_status};
   return launch_weighted(c, ws, (cudaStream_t)stream);

@@ -260,9 +260,9 @@ struct WeightedCall {
   int d, E, H, k, act, dtype, add_residual;
   int* dev_status;
 };
-size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, bool tiles);
+size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, int dtype, bool tiles);
 // tiles: the tensor-core kernel takes the shape
-bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, bool tiles);
+bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, int dtype, bool tiles);
 int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s);
 int launch_expand_mask(const uint32_t* mask_bits, void* rt, int64_t N, int E, int dtype,
                        cudaStream_t s);

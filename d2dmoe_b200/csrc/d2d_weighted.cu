@@ -11,9 +11,9 @@
 //           element, in a format of its own (encode8) that is off by 2^-14 of the largest of eight where bf16 would be by 2^-9; the
 //           general-shape kernel's are fp32.
 //   few     Calls of few pairs are bound by latency and by the weights' bytes: two kernels without lists, all
-//           sums in 32 bits.  The first splits every pair's hidden columns and, where there are fewer such pieces than SMs,
-//           the depth d over blocks; the second adds the depth's parts, applies bias, activation and weight, and takes
-//           the second product, the slots of a token split over a cluster whose sums meet in distributed shared memory.
+//           sums in 32 bits.  Blocks share out a pair's hidden columns in the first, a token's columns in the second;
+//           where those are fewer than the SMs take, clusters split the depth, or the slots, and meet in distributed
+//           shared memory.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -436,14 +436,11 @@ combine_coded_kernel(const uint16_t* __restrict__ y, const int32_t* __restrict__
 }
 
 // -- few pairs ---------------------------------------------------------------------------------------------
-// columns of a block: four threads of 16 bytes each, or 32 of one element
-template <int V>
-constexpr int few_threads = V == 1 ? 32 : 4;
-
+// TC threads side by side have V columns each of a block.  Sixteen of 16 bytes where the rows are that long: whole
+// 256-byte pieces of a row of the weights (64-byte pieces of W2's 4 KB rows took 14.5 us for one token, 4 MB).
 // V sums of each thread over the block's threads of the same columns -> the first TC V threads, in red
-template <int V>
+template <int V, int TC>
 __device__ __forceinline__ float few_sum(float (&v)[V], float* red) {
-  constexpr int TC = few_threads<V>;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
 #pragma unroll
   for (int o = TC; o < 32; o <<= 1)
@@ -461,33 +458,36 @@ __device__ __forceinline__ float few_sum(float (&v)[V], float* red) {
   return sum;
 }
 
-// part[s][p][gate, up][H]: pair p's share of x W1 (and x W_up) from depth part s
-template <typename T, int V, bool GLU>
+// hidden[p][H]: pair p's hidden values times its weight.  A cluster has TC V of them, its CTAs share the depth and meet in
+// distributed shared memory: blockIdx.x = (hidden columns, CTA of the cluster).
+template <typename T, int V, int TC, bool GLU>
 __global__ void __launch_bounds__(NT)
-few_hidden_kernel(WeightedCall c, int splits, float* __restrict__ part) {
-  constexpr int TC = few_threads<V>, RG = NT / TC, G = GLU ? 2 : 1;
+few_hidden_kernel(WeightedCall c, float* __restrict__ hidden) {
+  constexpr int RG = NT / TC;
   __shared__ float red[NT / 32 * TC * V];
-  grid_launch_dependents();
+  __shared__ float sums[2][TC * V];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
   grid_dependency_wait();
-  fresh(c.x, c.experts, c.w1, c.w_up);
+  grid_launch_dependents();                 // behind the wait: the next kernel relies on it
+  fresh(c.x, c.experts, c.weights, c.w1, c.b1, c.w_up);
   const int tid = threadIdx.x, H = c.H, d = c.d;
-  const int hcs = ceil_div(H, TC * V), hc = blockIdx.x % hcs, s = blockIdx.x / hcs;
-  const int64_t p = blockIdx.y, P = c.N * c.k, t = p / c.k;
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t p = blockIdx.y, t = p / c.k;
   const int e = c.experts[p];
-  if ((unsigned)e >= (unsigned)c.E) {
+  if ((unsigned)e >= (unsigned)c.E) {       // (all of a cluster)
     if (e != -1 && tid == 0) report(c.dev_status, D2D_ERR_INDEX_RANGE);
     return;
   }
-  const int depth = ceil_div(d, splits), d0 = s * depth, d1 = min(d, d0 + depth);
-  const int col = hc * TC * V + (tid % TC) * V;
-  const bool in = col < H;
+  const int depth = ceil_div(d, ctas), d0 = rank * depth, d1 = min(d, d0 + depth);
+  const int col0 = blockIdx.x / ctas * TC * V, col = col0 + (tid % TC) * V;
   const T* const x = (const T*)c.x + t * d;
   const T* const w1 = (const T*)c.w1 + (int64_t)e * d * H + col;
   const T* const wu = GLU ? (const T*)c.w_up + (int64_t)e * d * H + col : nullptr;
   float a[V], u[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) a[i] = u[i] = 0.f;
-  if (in)
+  if (col < H)
 #pragma unroll 4
     for (int r = d0 + tid / TC; r < d1; r += RG) {
       float f[V];
@@ -501,22 +501,48 @@ few_hidden_kernel(WeightedCall c, int splits, float* __restrict__ part) {
         for (int i = 0; i < V; ++i) u[i] = fmaf(xv, f[i], u[i]);
       }
     }
-  float* const to = part + ((int64_t)s * P + p) * G * H;
-  const int out = hc * TC * V + tid;
-  const float sum = few_sum<V>(a, red);
-  if (tid < TC * V && out < H) to[out] = sum;
-  if (GLU) {
-    const float up = few_sum<V>(u, red);
-    if (tid < TC * V && out < H) to[H + out] = up;
+  float sum = few_sum<V, TC>(a, red), up = GLU ? few_sum<V, TC>(u, red) : 1.f;
+  if (ctas > 1) {
+    if (tid < TC * V) sums[0][tid] = sum, sums[1][tid] = up;
+    cluster.sync();
+    if (rank == 0 && tid < TC * V) {
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < ctas) {
+          const float* const s = cluster.map_shared_rank(&sums[0][0], r);
+          sum += s[tid];
+          if (GLU) up += s[TC * V + tid];
+        }
+    }
   }
+  const int h = col0 + tid;
+  if (rank == 0 && tid < TC * V && h < H) {
+    if (c.b1) sum += DT<T>::to_f(((const T*)c.b1)[(int64_t)e * H + h]);
+    hidden[p * H + h] = activate(sum, c.act) * up * c.weights[p];
+  }
+  if (ctas > 1) cluster.sync();             // the others' sums are read until here
 }
 
-// A cluster has V few_threads columns of a token, a CTA of it `share` slots: blockIdx.x = (columns, CTA of the cluster).
-template <typename T, int V, bool GLU>
+// A cluster has TC V columns of a token, a CTA of it `share` slots: blockIdx.x = (columns, CTA of the cluster).
+// It starts when every block of the first kernel is past its own wait, so what came before that one is there: experts and W2
+// are read ahead of the wait for the hidden values, and the first rows' latency goes by meanwhile.
+template <typename T, int V>
+struct Raw {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float* f) const { load_row<T, V>(reinterpret_cast<const T*>(&v), f); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void get(float* f) const { f[0] = DT<T>::to_f(v); }
+};
+template <typename T, int V, int TC>
 __global__ void __launch_bounds__(NT)
-few_out_kernel(WeightedCall c, int splits, int share, const float* __restrict__ part) {
-  constexpr int TC = few_threads<V>, RG = NT / TC, G = GLU ? 2 : 1;
-  extern __shared__ float hs[];             // [share][H] hidden values times their weight, then [share] experts
+few_out_kernel(WeightedCall c, int share, const float* __restrict__ hidden) {
+  constexpr int RG = NT / TC, PRE = 8;
+  extern __shared__ float hs[];             // [share][H] hidden values, then [share] experts
   __shared__ float red[NT / 32 * TC * V];
   __shared__ float sums[TC * V];
   namespace cg = cooperative_groups;
@@ -526,76 +552,93 @@ few_out_kernel(WeightedCall c, int splits, int share, const float* __restrict__ 
   const int j0 = rank * share, js = max(0, min(share, k - j0));          // my slots
   int* const es = reinterpret_cast<int*>(hs + share * H);
   grid_launch_dependents();
-  grid_dependency_wait();
-  fresh(c.x, c.experts, c.weights, c.b1, c.w2, c.last_bias, part);
-  const int64_t t = blockIdx.y, P = c.N * k;
+  const int64_t t = blockIdx.y;
   for (int j = tid; j < js; j += NT) {
     const int e = c.experts[t * k + j0 + j];
     es[j] = (unsigned)e < (unsigned)c.E ? e : -1;
   }
   __syncthreads();
+  const int col0 = blockIdx.x / ctas * TC * V, col = col0 + (tid % TC) * V, rows = col < d ? js * H : 0;
+  // row r of my slots: hidden column h of slot j
+  Raw<T, V> pre[PRE];
+  int j = 0, h = tid / TC;
+#pragma unroll
+  for (int i = 0; i < PRE; ++i) {
+    while (h >= H) h -= H, ++j;
+    if (tid / TC + i * RG < rows && es[j] >= 0) pre[i].load((const T*)c.w2 + ((int64_t)es[j] * H + h) * d + col);
+    h += RG;
+  }
+  grid_dependency_wait();
+  fresh(c.x, c.last_bias, hidden);
   for (int i = tid; i < js * H; i += NT) {
-    const int j = i / H, h = i - j * H, e = es[j];
-    float v = 0.f;
-    if (e >= 0) {
-      const float* q = part + (t * k + j0 + j) * G * H + h;
-      float up = 0.f;
-#pragma unroll 8
-      for (int s = 0; s < splits; ++s) {
-        v += q[s * P * G * H];
-        if (GLU) up += q[s * P * G * H + H];
-      }
-      if (c.b1) v += DT<T>::to_f(((const T*)c.b1)[(int64_t)e * H + h]);
-      v = activate(v, c.act);
-      if (GLU) v *= up;
-      v *= c.weights[t * k + j0 + j];
-    }
-    hs[i] = v;
+    const bool there = es[i / H] >= 0;
+    hs[i] = there ? hidden[(t * k + j0) * H + i] : 0.f;
   }
   __syncthreads();
-  const int col0 = blockIdx.x / ctas * TC * V, col = col0 + (tid % TC) * V;
-  float a[V];
+  float a[V], f[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) a[i] = 0.f;
-  if (col < d)
-    for (int j = 0; j < js; ++j) {
-      const int e = es[j];
-      if (e < 0) continue;
-      const T* const w2 = (const T*)c.w2 + (int64_t)e * H * d + col;
-#pragma unroll 4
-      for (int h = tid / TC; h < H; h += RG) {
-        float f[V];
-        load_row<T, V>(w2 + (int64_t)h * d, f);
-        const float hv = hs[j * H + h];
+  j = 0, h = tid / TC;
 #pragma unroll
-        for (int q = 0; q < V; ++q) a[q] = fmaf(hv, f[q], a[q]);
-      }
+  for (int i = 0; i < PRE; ++i) {
+    while (h >= H) h -= H, ++j;
+    const int r = tid / TC + i * RG;
+    if (r < rows && es[j] >= 0) {
+      pre[i].get(f);
+#pragma unroll
+      for (int q = 0; q < V; ++q) a[q] = fmaf(hs[r], f[q], a[q]);
     }
-  float sum = few_sum<V>(a, red);
-  if (tid < TC * V) sums[tid] = sum;
-  cluster.sync();
-  if (rank == 0 && tid < TC * V && col0 + tid < d) {
-    for (int r = 1; r < ctas; ++r) sum += cluster.map_shared_rank(sums, r)[tid];
-    const int at = col0 + tid;
+    h += RG;
+  }
+  while (h >= H) h -= H, ++j;
+  for (; j < js && col < d; ++j, h -= H) {
+    const int e = es[j];
+    if (e < 0) {
+      if (h < H) h += (H - h + RG - 1) / RG * RG;
+      continue;
+    }
+    const T* const w2 = (const T*)c.w2 + (int64_t)e * H * d + col;
+#pragma unroll 4
+    for (; h < H; h += RG) {
+      load_row<T, V>(w2 + (int64_t)h * d, f);
+      const float hv = hs[j * H + h];
+#pragma unroll
+      for (int q = 0; q < V; ++q) a[q] = fmaf(hv, f[q], a[q]);
+    }
+  }
+  float sum = few_sum<V, TC>(a, red);
+  if (ctas > 1) {
+    if (tid < TC * V) sums[tid] = sum;
+    cluster.sync();
+    if (rank == 0 && tid < TC * V) {
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < ctas) sum += cluster.map_shared_rank(sums, r)[tid];
+    }
+  }
+  const int at = col0 + tid;
+  if (rank == 0 && tid < TC * V && at < d) {
     if (c.last_bias) sum += DT<T>::to_f(((const T*)c.last_bias)[at]);
     if (c.add_residual) sum += DT<T>::to_f(((const T*)c.x)[t * d + at]);
     ((T*)c.out)[t * d + at] = DT<T>::from_f(sum);
   }
-  cluster.sync();                           // the others' sums are read until here
+  if (ctas > 1) cluster.sync();             // the others' sums are read until here
 }
 
 // -- host ----------------------------------------------------------------------------------------------------
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-bool takes_few(int64_t P, int d, int H, int k) {
-  return P <= 64 && (size_t)k * H * sizeof(float) <= 64 * 1024;
+// The first form reads its expert for every pair, out of L2 where all of them fit; lists read each expert once or twice, but
+// have three more kernels and wait for a first tile.  Few / lists, us: 2048 x 128 gated, 128 experts (1.6 MB each) 16
+// tokens x 8 34 / 58, 37 tokens 59 / 60, 48 tokens 84 / 61; 768 x 128, 24 experts (393 KB) 48 tokens x 4 14 / 17, 64 tokens
+// 16.5 / 16.6, 96 tokens 20 / 16.5; 768 x 32 (98 KB) 197 tokens x 4 15 / 21.  Where lists mean the general-shape kernel:
+// fp32 768 x 128 (786 KB) 256 tokens x 4 74 / 128, 400 tokens 111 / 119.
+bool takes_few(int64_t P, int d, int E, int H, int k, bool glu, int dtype, bool tiles) {
+  const int64_t expert = (int64_t)(glu ? 3 : 2) * d * H * (dtype == D2D_F32 ? 4 : 2);
+  const int64_t most = tiles ? std::max<int64_t>(100 << 20, expert * E * 9 / 4) : 1200LL << 20;
+  return P <= 2048 && P * expert <= most && (size_t)k * H * sizeof(float) <= 64 * 1024;
 }
-int few_splits(int64_t P, int d, int H, int V) {
-  const int64_t pieces = P * ceil_div(H, (V == 1 ? 32 : 4) * V);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(16, d / 128), 296 / pieces));
-}
-constexpr int MOST_SPLITS = 16;
 
 // Pairs of a thread in the sort: 4 up to 256 blocks of 1024 pairs, 16 beyond (fewer rows of counts for every block to add up;
 // past a million pairs they grow again).
@@ -625,30 +668,41 @@ Layout layout_of(int64_t P, int d, int E, bool tiles) {
   return l;
 }
 
-template <typename T, int V, bool GLU>
-int few(const WeightedCall& c, float* part, cudaStream_t s) {
+template <typename T, int V, int TC, bool GLU>
+int few_hidden(const WeightedCall& c, float* hidden, cudaStream_t s) {
+  // CTAs of a cluster: 128 rows of the depth each at least, unless there are blocks enough
   const int64_t P = c.N * c.k;
-  const int splits = few_splits(P, c.d, c.H, V), cols = few_threads<V> * V;
-  // CTAs of a cluster: a slot each, unless there are blocks enough
-  const int64_t blocks = (int64_t)ceil_div(c.d, cols) * c.N;
+  const int pieces = ceil_div(c.H, TC * V);
   int ctas = 1;
-  while (ctas < 8 && 2 * ctas <= c.k && 2 * ctas * blocks <= 1024) ctas *= 2;
+  while (ctas < 8 && 256 * ctas <= c.d && 2 * ctas * pieces * P <= 592) ctas *= 2;
+  return launch_pdl_cluster(ctas, few_hidden_kernel<T, V, TC, GLU>, dim3((unsigned)(pieces * ctas), (unsigned)P), dim3(NT), 0,
+                            s, c, hidden);
+}
+template <typename T, int V, int TC>
+int few_out(const WeightedCall& c, const float* hidden, cudaStream_t s) {
+  // CTAs of a cluster: a slot each, unless there are blocks enough
+  const int pieces = ceil_div(c.d, TC * V);
+  int ctas = 1;
+  while (ctas < 8 && 2 * ctas <= c.k && 2 * ctas * pieces * c.N <= 592) ctas *= 2;
   const int share = ceil_div(c.k, ctas);
   const size_t smem = ((size_t)share * c.H + share) * sizeof(float);
-  int rc = device_launch_facts((const void*)few_out_kernel<T, V, GLU>, smem, nullptr);
+  const auto k = few_out_kernel<T, V, TC>;
+  const int rc = device_launch_facts((const void*)k, smem, nullptr);
   if (rc != D2D_OK) return rc;
-  rc = launch_pdl(few_hidden_kernel<T, V, GLU>, dim3((unsigned)(ceil_div(c.H, cols) * splits), (unsigned)P), dim3(NT),
-                  0, s, c, splits, part);
+  return launch_pdl_cluster(ctas, k, dim3((unsigned)(pieces * ctas), (unsigned)c.N), dim3(NT), smem, s, c, share, hidden);
+}
+template <typename T, int V>
+int few(const WeightedCall& c, float* hidden, cudaStream_t s) {
+  constexpr int WIDE = V == 1 ? 32 : 16, NARROW = V == 1 ? 32 : 4;
+  const int rc = c.w_up ? few_hidden<T, V, NARROW, true>(c, hidden, s) : few_hidden<T, V, NARROW, false>(c, hidden, s);
   if (rc != D2D_OK) return rc;
-  return launch_pdl_cluster(ctas, few_out_kernel<T, V, GLU>, dim3((unsigned)(ceil_div(c.d, cols) * ctas), (unsigned)c.N),
-                            dim3(NT), smem, s, c, splits, share, (const float*)part);
+  return c.d >= 4 * WIDE * V ? few_out<T, V, WIDE>(c, hidden, s) : few_out<T, V, NARROW>(c, hidden, s);
 }
 template <typename T>
-int few_t(const WeightedCall& c, float* part, cudaStream_t s) {
+int few_t(const WeightedCall& c, float* hidden, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = c.H % V == 0 && c.d % V == 0 && al16(c.w1) && al16(c.w_up) && al16(c.w2);
-  if (c.w_up) return vec ? few<T, V, true>(c, part, s) : few<T, 1, true>(c, part, s);
-  return vec ? few<T, V, false>(c, part, s) : few<T, 1, false>(c, part, s);
+  return vec ? few<T, V>(c, hidden, s) : few<T, 1>(c, hidden, s);
 }
 
 template <typename T, int V>
@@ -676,15 +730,15 @@ int combine_coded(const WeightedCall& c, const void* y, int sms, cudaStream_t s)
 
 }  // namespace
 
-size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, bool tiles) {
+size_t weighted_workspace_bytes(int64_t N, int d, int E, int H, int k, bool glu, int dtype, bool tiles) {
   const int64_t P = N * k;
-  if (takes_few(P, d, H, k)) return up256((size_t)MOST_SPLITS * P * (glu ? 2 : 1) * H * sizeof(float));
+  if (takes_few(P, d, E, H, k, glu, dtype, tiles)) return up256((size_t)P * H * sizeof(float));
   return layout_of(P, d, E, tiles).total;
 }
 
-bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, bool tiles) {
+bool weighted_supported(int64_t N, int d, int E, int H, int k, bool glu, int dtype, bool tiles) {
   return E <= MAX_E && k <= 32 && N * k < 0x7fffffffLL &&
-         (tiles || takes_few(N * k, d, H, k) || experts_simt_fits(H, glu));
+         (tiles || takes_few(N * k, d, E, H, k, glu, dtype, tiles) || experts_simt_fits(H, glu));
 }
 
 int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s) {
@@ -692,7 +746,7 @@ int launch_weighted(const WeightedCall& c, void* ws, cudaStream_t s) {
   int rc = device_launch_facts(nullptr, 0, &sms);
   if (rc != D2D_OK) return rc;
   const int64_t P = c.N * c.k;
-  if (takes_few(P, c.d, c.H, c.k))
+  if (takes_few(P, c.d, c.E, c.H, c.k, c.w_up != nullptr, c.dtype, c.packed != nullptr))
     return c.dtype == D2D_F32 ? few_t<float>(c, (float*)ws, s) : few_t<bf16>(c, (float*)ws, s);
   const Layout l = layout_of(P, c.d, c.E, c.packed != nullptr);
   uint8_t* const base = (uint8_t*)ws;

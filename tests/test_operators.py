@@ -475,6 +475,12 @@ EXPERTS = [
     (513, 768, 24, 128, 1, "bf16", False, True, "gelu"), (700, 200, 9, 40, 4, "fp32", True, False, "gelu"),
     (1100, 768, 12, 32, 12, "bf16", False, True, "gelu"), (1500, 512, 128, 128, 8, "bf16", True, False, "gelu_tanh"),
     (1400, 101, 200, 7, 32, "fp32", False, True, "relu"), (5000, 128, 24, 64, 4, "bf16", False, True, "relu"),
+    # either side of the line between the two forms (2048 pairs, or the experts' bytes), lists of one chunk and of several
+    (682, 64, 3, 16, 3, "bf16", False, True, "leaky_relu"), (683, 64, 3, 16, 3, "bf16", False, True, "leaky_relu"),
+    (900, 130, 7, 20, 3, "bf16", False, True, "gelu"), (2049, 200, 2, 50, 1, "fp32", True, False, "tanh"),
+    (36, 2048, 128, 128, 8, "bf16", True, False, "gelu"), (38, 2048, 128, 128, 8, "bf16", True, False, "gelu"),
+    (66, 768, 24, 128, 4, "bf16", False, True, "relu"), (70, 768, 24, 128, 4, "bf16", False, True, "relu"),
+    (700, 3008, 4, 300, 3, "bf16", False, True, "gelu"), (33000, 64, 120, 16, 8, "bf16", False, True, "relu"),
 ]
 
 
@@ -498,7 +504,7 @@ def test_weighted_experts(case):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N", [5, 400])
+@pytest.mark.parametrize("N", [5, 400])             # 30 pairs, 2400 pairs
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_weighted_experts_odd_choices(N, dtype):
     """Slots without an expert, tokens without any, the same expert in several slots, weights of zero, negative and NaN,
@@ -550,7 +556,7 @@ def test_weighted_experts_sizes_and_infinities():
     """Outputs of very different sizes beside each other, tiny, huge and zero rows; infinities and NaN stay what they are
     in their own columns."""
     import d2dmoe_b200 as D
-    x, e, w, w1, b1, w2, up, lb = experts_case(300, 128, 12, 32, 3, "bf16", False, True, seed=4)
+    x, e, w, w1, b1, w2, up, lb = experts_case(900, 128, 12, 32, 3, "bf16", False, True, seed=4)
     e[:, 0], e[:, 1], e[:, 2] = 0, 1, 2
     w2[0] *= torch.logspace(-30, 30, 128, device="cuda").to(w2.dtype)
     w2[1] *= 1e-36
@@ -582,25 +588,25 @@ def test_weighted_experts_sizes_and_infinities():
 @pytest.mark.gpu
 def test_weighted_experts_strided_and_misaligned():
     import d2dmoe_b200 as D
-    x, e, w, w1, b1, w2, up, lb = experts_case(200, 128, 12, 32, 4, "bf16", False, True, seed=2)
+    x, e, w, w1, b1, w2, up, lb = experts_case(600, 128, 12, 32, 4, "bf16", False, True, seed=2)
     packed = D.ops.prepack_experts(w1, b1, w2)
     want, tol = experts_reference(x, e, w, w1, b1, w2, "relu", None, lb)
-    wide = torch.zeros(200, 140, dtype=x.dtype, device="cuda")
+    wide = torch.zeros(600, 140, dtype=x.dtype, device="cuda")
     wide[:, 3:131] = x
-    off = torch.zeros(200 * 128 + 1, dtype=x.dtype, device="cuda")[1:].view(200, 128)
+    off = torch.zeros(600 * 128 + 1, dtype=x.dtype, device="cuda")[1:].view(600, 128)
     off.copy_(x)
-    ew = torch.full((200, 9), -1, dtype=torch.int32, device="cuda")
+    ew = torch.full((600, 9), -1, dtype=torch.int32, device="cuda")
     ew[:, 2:6] = e
     lbo = torch.zeros(129, dtype=x.dtype, device="cuda")[1:]
     lbo.copy_(lb)
-    for n in (200, 9):
+    for n in (600, 9):
         for xx, bias in ((wide[:, 3:131], lb), (off, lb), (x, lbo)):
             got = D.ops.experts_weighted(xx[:n], ew[:n, 2:6], w.t().contiguous().t()[:n], w1, b1, w2, "relu",
                                          packed=packed, last_bias=bias)
             within(got, want[:n], tol[:n], "strides")
-    batch = D.ops.experts_weighted(x.view(4, 50, 128), e.view(4, 50, 4), w.view(4, 50, 4), w1, b1, w2, "relu",
+    batch = D.ops.experts_weighted(x.view(4, 150, 128), e.view(4, 150, 4), w.view(4, 150, 4), w1, b1, w2, "relu",
                                    packed=packed, last_bias=lb)
-    assert torch.equal(batch.view(200, 128), D.ops.experts_weighted(x, e, w, w1, b1, w2, "relu", packed=packed,
+    assert torch.equal(batch.view(600, 128), D.ops.experts_weighted(x, e, w, w1, b1, w2, "relu", packed=packed,
                                                                      last_bias=lb))
 
 
@@ -800,7 +806,7 @@ def test_weighted_experts_give_up_on_a_withheld_tile():
     """A weight tile that never comes: the bounded wait runs out, the status says so, and the next call is whole."""
     import d2dmoe_b200 as D
     from d2dmoe_b200 import _capi
-    x, e, w, w1, b1, w2, up, lb = experts_case(400, 128, 12, 32, 4, "bf16", False, True)
+    x, e, w, w1, b1, w2, up, lb = experts_case(700, 128, 12, 32, 4, "bf16", False, True)
     packed = D.ops.prepack_experts(w1, b1, w2)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     _capi.lib.d2d_debug_configure(10, 1)
@@ -863,14 +869,14 @@ def test_refusals_at_the_c_abi():
         assert rback(**kw) == BAD, kw
     assert rback(E=1025) == UNS and rback(E=64, k=33) == UNS and rback(dt=2) == UNS
 
-    def ws_bytes(N=400, d=128, E=12, H=32, k=4, glu=0, packed=0, dt=1):
+    def ws_bytes(N=4000, d=128, E=12, H=32, k=4, glu=0, packed=0, dt=1):
         rc = lib.d2d_experts_weighted_workspace_bytes(N, d, E, H, k, glu, packed, dt, C.byref(n))
         return rc if rc else n.value
     need = ws_bytes()
-    assert need >= 400 * 4 * 128 * 4 > ws_bytes(packed=1) >= 400 * 4 * 128 * 2 and ws_bytes(N=0) >= 0
+    assert need >= 4000 * 4 * 128 * 4 > ws_bytes(packed=1) >= 4000 * 4 * 128 * 2 and ws_bytes(N=0) >= 0
     assert ws_bytes(N=-1) == BAD and ws_bytes(k=13) == BAD and ws_bytes(dt=9) == UNS
 
-    def experts(x=a, e=a, w=a, w1=a, w2=a, out=a, res=0, N=400, d=128, E=12, H=32, k=4, act=0, dt=1, ws=a, nb=None):
+    def experts(x=a, e=a, w=a, w1=a, w2=a, out=a, res=0, N=4000, d=128, E=12, H=32, k=4, act=0, dt=1, ws=a, nb=None):
         return lib.d2d_experts_weighted(x, e, w, w1, None, None, w2, None, None, res, out, N, d, E, H, k, act, dt, ws,
                                         need if nb is None else nb, None, None)
     assert experts(N=0) == OKAY
