@@ -778,6 +778,52 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// What both calls of the weighted experts share: weights as addresses and sizes.
+struct ExpertWeights {
+  const void *w1, *b1, *up, *w2, *packed;
+  int64_t E, d, H;
+  int act;
+  at::ScalarType dtype;
+};
+
+PyObject* run_weighted_experts(const ExpertWeights& m, const at::Tensor& xt, const at::Tensor& et, const at::Tensor& wt,
+                               const at::Tensor* bias, bool residual, const at::Tensor* status) {
+  const int dt = dtype_of(xt);
+  of_type(xt, m.dtype, "x");
+  of_type(et, at::kInt, "experts");
+  of_type(wt, at::kFloat, "weights");
+  TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) == m.d, "x must be [.., ", m.d, "]");
+  const int64_t N = xt.numel() / m.d;
+  TORCH_CHECK_VALUE(et.dim() == xt.dim() && et.sizes().slice(0, et.dim() - 1) == xt.sizes().slice(0, xt.dim() - 1) &&
+                        wt.sizes() == et.sizes(),
+                    "experts and weights must be [.., k] for x [.., d]");
+  const int64_t k = et.size(-1);
+  if (bias) {
+    of_type(*bias, xt.scalar_type(), "last_bias");
+    TORCH_CHECK_VALUE(bias->numel() == m.d && bias->is_contiguous(), "last_bias must have ", m.d, " values");
+  }
+  if (k < 1 || k > m.E) return PyLong_FromLong(D2D_ERR_BAD_ARG);
+  On on(xt);
+  const auto aligned = [](at::Tensor t) {      // (views may start anywhere)
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+  };
+  const at::Tensor x = aligned(xt.contiguous()), e = et.contiguous(), w = wt.contiguous();
+  const at::Tensor lb = bias ? aligned(*bias) : at::Tensor();
+  at::Tensor out = at::detail::empty_cuda(xt.sizes(), xt.options().requires_grad(c10::nullopt)), ws;
+  size_t bytes = 0;
+  int rc = d2d_experts_weighted_workspace_bytes(N, (int)m.d, (int)m.E, (int)m.H, (int)k, m.up != nullptr,
+                                                m.packed != nullptr, dt, &bytes);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  if (N > 0) {
+    ws = at::detail::empty_cuda({(int64_t)bytes}, xt.options().dtype(at::kByte));
+    rc = d2d_experts_weighted(x.data_ptr(), (const int32_t*)e.data_ptr(), (const float*)w.data_ptr(), m.w1, m.b1, m.up,
+                              m.w2, m.packed, data_or_null(&lb), residual, out.data_ptr(), N, (int)m.d, (int)m.E,
+                              (int)m.H, (int)k, m.act, dt, ws.data_ptr(), bytes, (int*)data_or_null(status), on.stream);
+  }
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap(out);
+}
+
 // experts_weighted(x [.., d], experts [.., k], weights [.., k], w1, b1 | None, w_up | None, w2, packed | None,
 //                  last bias | None, residual, act, status | None) -> out
 PyObject* experts_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -797,16 +843,8 @@ PyObject* experts_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor* status = given(a[11], "status", &xt);
   if (PyErr_Occurred()) return nullptr;
   const int dt = dtype_of(xt);
-  of_type(et, at::kInt, "experts");
-  of_type(wt, at::kFloat, "weights");
   TORCH_CHECK_VALUE(w1.dim() == 3 && w1.numel() > 0, "w1 must be [experts, d, expert width]");
   const int64_t E = w1.size(0), d = w1.size(1), H = w1.size(2);
-  TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) == d, "x must be [.., ", d, "]");
-  const int64_t N = xt.numel() / d;
-  TORCH_CHECK_VALUE(et.dim() == xt.dim() && et.sizes().slice(0, et.dim() - 1) == xt.sizes().slice(0, xt.dim() - 1) &&
-                        wt.sizes() == et.sizes(),
-                    "experts and weights must be [.., k] for x [.., d]");
-  const int64_t k = et.size(-1);
   const auto weight = [&](const at::Tensor& t, const char* name, at::IntArrayRef shape) {
     of_type(t, xt.scalar_type(), name);
     TORCH_CHECK_VALUE(t.sizes() == shape && t.is_contiguous(), name, " must be contiguous, of shape ", shape);
@@ -815,36 +853,41 @@ PyObject* experts_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
   weight(w2, "w2", {E, H, d});
   if (b1) weight(*b1, "b1", {E, H});
   if (up) weight(*up, "w_up", {E, d, H});
-  if (bias) {
-    of_type(*bias, xt.scalar_type(), "last_bias");
-    TORCH_CHECK_VALUE(bias->numel() == d && bias->is_contiguous(), "last_bias must have ", d, " values");
-  }
   if (packed) {
     size_t most = 0;
     const int rc = d2d_prepack_experts_bytes((int)d, (int)E, (int)H, up != nullptr, dt, &most);
     TORCH_CHECK_VALUE(rc == D2D_OK && most > 0 && packed->is_contiguous() && packed->nbytes() >= most,
                       "packed weights are not those of this shape");
   }
-  if (k < 1 || k > E) return PyLong_FromLong(D2D_ERR_BAD_ARG);
-  On on(xt);
-  const auto aligned = [](at::Tensor t) {      // (views may start anywhere)
-    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
-  };
-  const at::Tensor x = aligned(xt.contiguous()), e = et.contiguous(), w = wt.contiguous();
-  const at::Tensor lb = bias ? aligned(*bias) : at::Tensor();
-  at::Tensor out = at::detail::empty_cuda(xt.sizes(), xt.options()), ws;
-  size_t bytes = 0;
-  int rc = d2d_experts_weighted_workspace_bytes(N, (int)d, (int)E, (int)H, (int)k, up != nullptr, packed != nullptr, dt, &bytes);
-  if (rc != D2D_OK) return PyLong_FromLong(rc);
-  if (N > 0) {
-    ws = at::detail::empty_cuda({(int64_t)bytes}, xt.options().dtype(at::kByte));
-    rc = d2d_experts_weighted(x.data_ptr(), (const int32_t*)e.data_ptr(), (const float*)w.data_ptr(), w1.data_ptr(),
-                              data_or_null(b1), data_or_null(up), w2.data_ptr(), data_or_null(packed),
-                              data_or_null(&lb), residual, out.data_ptr(), N, (int)d, (int)E, (int)H, (int)k, act, dt,
-                              ws.data_ptr(), bytes, (int*)data_or_null(status), on.stream);
+  const ExpertWeights m = {w1.data_ptr(), data_or_null(b1), data_or_null(up), w2.data_ptr(), data_or_null(packed),
+                           E, d, H, act, w1.scalar_type()};
+  return run_weighted_experts(m, xt, et, wt, bias, residual, status);
+  END_HANDLE_TH_ERRORS
+}
+
+// run_weighted(plan, modules, parameters, attributes, x, experts, weights, last bias | None, residual, status)
+//   -> out | status code (int) | None: the plan is stale.  The plan's module is the experts'.
+PyObject* run_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "run_weighted takes 10 arguments");
+  Plan* p = static_cast<Plan*>(PyCapsule_GetPointer(a[0], kPlan));
+  if (!p) return nullptr;
+  if (!still_valid(*p, a + 1)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
   }
-  if (rc != D2D_OK) return PyLong_FromLong(rc);
-  return wrap(out);
+  const at::Tensor& xt = needed(a[4], "x");
+  TORCH_CHECK_VALUE(xt.device() == p->device, "tensors of one call live on different devices: ", p->device, " and ",
+                    xt.device(), " (x)");
+  const at::Tensor& et = needed(a[5], "experts", &xt);
+  const at::Tensor& wt = needed(a[6], "weights", &xt);
+  const at::Tensor* bias = given(a[7], "last_bias", &xt);
+  const int residual = PyObject_IsTrue(a[8]);
+  const at::Tensor* status = given(a[9], "status", &xt);
+  if (PyErr_Occurred()) return nullptr;
+  use_on(*p, c10::cuda::getCurrentCUDAStream(p->device.index()));
+  const ExpertWeights m = {p->w1, p->b1, p->wup, p->w2, p->ep, p->E, p->d, p->H, (int)p->act, p->dtype};
+  return run_weighted_experts(m, xt, et, wt, bias, residual, status);
   END_HANDLE_TH_ERRORS
 }
 
@@ -854,6 +897,7 @@ PyMethodDef kMethods[] = {
     {"route", (PyCFunction)(void (*)(void))route, METH_FASTCALL, nullptr},
     {"route_backward", (PyCFunction)(void (*)(void))route_backward, METH_FASTCALL, nullptr},
     {"experts_weighted", (PyCFunction)(void (*)(void))experts_weighted, METH_FASTCALL, nullptr},
+    {"run_weighted", (PyCFunction)(void (*)(void))run_weighted, METH_FASTCALL, nullptr},
     {"mark", (PyCFunction)(void (*)(void))mark, METH_FASTCALL, nullptr},
     {"wait_mark", (PyCFunction)(void (*)(void))wait_mark, METH_FASTCALL, nullptr},
     {"make_pipe", (PyCFunction)(void (*)(void))make_pipe, METH_FASTCALL, nullptr},

@@ -257,19 +257,66 @@ class B200KernelExperts(ExpertsLayer):
         self._packed.invalidate()
 
     # -- weighted form --------------------------------------------------------------------
-    @torch.no_grad()
     def forward_weighted(self, x, experts, weights, last_bias=None, add_residual=False):
         """``last_bias (+ x) + sum_j weights[.., j] * expert_{experts[.., j]}(x)`` for x [.., d] and what
         ``route_tokens`` returns: experts [.., k] int32 (-1: no such slot), weights [.., k] fp32.  A token's sum is held in
-        fp32, in the order of its slots, and rounded once.  (Upstream multiplies every expert's output by its
-        routing entry, architectures/moe/moe_layers.py:91-101.)"""
+        fp32, in the order of its slots, and rounded once; the result has no gradient.  (Upstream multiplies every
+        expert's output by its routing entry, architectures/moe/moe_layers.py:91-101.)"""
         self._check_mode()
         if self._capture is not None:
             raise NotImplementedError("activation norms are captured in the unweighted forms")
+        state = self.__dict__
+        if last_bias is not None:
+            last_bias = last_bias.detach()
+        status = self._status_words()[x.device] if x.is_cuda else None
+        plan = state.get("_weighted_plan")           # (not there in modules saved whole before it was)
+        if plan is None:
+            plan = state["_weighted_plan"] = _Plan()
+        with_plan = 2 if x.is_cuda else 0
+        for _ in range(with_plan):
+            if plan.handle is not None:
+                r = host.run_weighted(plan.handle, self._modules, self._parameters, state, x, experts, weights,
+                                      last_bias, add_residual, status)
+                if type(r) is int:
+                    raise D2DError(r, "d2d_experts_weighted")
+                if r is not None:
+                    return r
+            with torch.no_grad():
+                plan.handle = self._make_weighted_plan()
+            if plan.handle is None:
+                break
+        with torch.no_grad():
+            p = self.kernel_params()
+            return ops.experts_weighted(x, experts, weights, p["w1"], p["b1"], p["w2"], p["act"], w_up=p["w_up"],
+                                        packed=self.packed(), last_bias=last_bias, add_residual=add_residual,
+                                        status=status)
+
+    def _make_weighted_plan(self):
+        """Plan of ``forward_weighted`` for the parameters as they are now, or None where something but the plain
+        parameters of this file hands them out (see MoeficationMoE._make_plan)."""
+        params = getattr(type(self), "kernel_params", None)
+        if (params not in (B200KernelExperts.kernel_params, B200GluExperts.kernel_params)
+                or type(self).packed is not B200KernelExperts.packed):
+            return None
         p = self.kernel_params()
-        return ops.experts_weighted(x, experts, weights, p["w1"], p["b1"], p["w2"], p["act"], w_up=p["w_up"],
-                                    packed=self.packed(), last_bias=last_bias, add_residual=add_residual,
-                                    status=self._status_words()[x.device])
+        links = [(2, "activation_str")]
+        if params is B200GluExperts.kernel_params:
+            links.append((0, "layers"))
+            for i in ("0", "1", "2"):
+                links += [(self.layers._modules, i), (self.layers._modules[i]._parameters, "w")]
+        else:
+            links += [(1, k) for k in ("w1", "b1", "w2")]
+        roots = (self._modules, self._parameters, self.__dict__)
+        slots = {id((roots[h] if type(h) is int else h).get(key)) for h, key in links}
+        w1 = p["w1"]
+        weights = [t for t in (w1, p["b1"], p["w_up"], p["w2"]) if t is not None]
+        if not w1.is_cuda or not all(id(t) in slots and t.dtype == w1.dtype and t.device == w1.device
+                                     and t.is_contiguous() for t in weights):
+            return None
+        packed = self.packed()
+        links.append((self._packed.__dict__, "_buf"))            # invalidate_packed() empties the slot
+        return host.make_plan(links, None, (w1, p["b1"], p["w_up"], p["w2"], packed, self._packed.mark), None,
+                              ACT[p["act"]], self._modules, self._parameters, self.__dict__)
 
     def _status_words(self):
         words = self.__dict__.get("_statuses")       # (not there in modules saved whole before it was)

@@ -668,6 +668,62 @@ def test_layer_in_weighted_mode(dtype, glu, residual, shape, routing):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("glu", [False, True])
+def test_weighted_call_follows_its_module(glu):
+    """What a call keeps of its module is checked by the next one: new values, new storage, another activation, dropped
+    packed weights, a copy of the module, another stream; and it refuses what it cannot serve."""
+    import copy
+    import d2dmoe_b200 as D
+    ex = weighted_layer(glu=glu).experts
+    for N in (6, 900):
+        g = gen(N)
+        x = randn(g, N, 256).bfloat16()
+        w, e = D.route_tokens(randn(g, N, 24), 4)
+
+        def check(what):
+            p = {n: t.detach() if torch.is_tensor(t) else t for n, t in ex.kernel_params().items()}
+            want = experts_reference(x, e, w, p["w1"], p["b1"], p["w2"], p["act"], p["w_up"])
+            within(ex.forward_weighted(x, e, w), *want, what)
+        check("first")
+        first = ex.kernel_params()["w1"]
+        with torch.no_grad():
+            first.mul_(-1.0)
+        check("values")
+        if glu:
+            ex.layers[1].w = torch.nn.Parameter(ex.layers[1].w.detach().flip(0).contiguous())
+        else:
+            ex.w2 = torch.nn.Parameter(ex.w2.detach().flip(0).contiguous())
+        check("storage")
+        ex.activation_str = "relu"
+        check("activation")
+        ex.activation_str = "gelu"
+        first.data.mul_(2.0)
+        ex.invalidate_packed()
+        check("written past the version counter")
+        other = copy.deepcopy(ex)
+        assert torch.equal(other.forward_weighted(x, e, w), ex.forward_weighted(x, e, w))
+        s = torch.cuda.Stream()
+        with torch.no_grad():
+            first.mul_(0.5)
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            check("stream")
+        torch.cuda.synchronize()
+        with pytest.raises(TypeError):
+            ex.forward_weighted(x.float(), e, w)
+        with pytest.raises(ValueError):
+            ex.forward_weighted(x[:, :128], e, w)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            ex.forward_weighted(x.cpu(), e, w)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            ex.forward_weighted(x, e.cpu(), w)
+        assert not ex.forward_weighted(x.clone().requires_grad_(), e, w).requires_grad
+    ex.capture_norms("output")
+    with pytest.raises(NotImplementedError):
+        ex.forward_weighted(x, e, w)
+
+
+@pytest.mark.gpu
 def test_routing_gradient_trains_a_router_of_dense_experts():
     """The weights' gradient through a mixture that torch computes: experts frozen, router and norm learn."""
     import d2dmoe_b200 as D
