@@ -21,6 +21,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -611,61 +613,51 @@ int param_code(at::ScalarType t, int x) {
   return t == at::ScalarType::Undefined ? x : t == at::kFloat ? D2D_F32 : D2D_BF16;
 }
 
-// layer_norm(x, weight | None, bias | None, eps, kind, weight offset, statistics wanted) -> (y, mean | None, rstd | None)
-PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 7, "layer_norm takes 7 arguments");
-  const at::Tensor& xt = needed(a[0], "x");
+// The operators themselves, without Python (autograd's threads call them too): status code, outputs by reference.
+// (Tensors without rows have no address; arguments are checked all the same.)
+void* address(const at::Tensor& t) {
+  static double none;
+  return t.numel() ? t.data_ptr() : &none;
+}
+
+struct NormHow {
+  double eps, offset;
+  int kind;
+};
+
+int norm_forward(const at::Tensor& xt, const at::Tensor* wt, const at::Tensor* bt, const NormHow& h, bool stats,
+                 at::Tensor* y, at::Tensor* mean, at::Tensor* rstd) {
   const int dt = dtype_of(xt);
   TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) > 0, "x must have rows of one value or more");
   const int64_t d = xt.size(-1);
   at::ScalarType pt = at::ScalarType::Undefined;
-  const at::Tensor w = param_of(given(a[1], "weight", &xt), "weight", d, xt.scalar_type(), &pt);
-  const at::Tensor b = param_of(given(a[2], "bias", &xt), "bias", d, xt.scalar_type(), &pt);
-  const double eps = PyFloat_AsDouble(a[3]);
-  const int kind = (int)PyLong_AsLong(a[4]);
-  const double offset = PyFloat_AsDouble(a[5]);
-  const int stats = PyObject_IsTrue(a[6]);
-  if (PyErr_Occurred()) return nullptr;
-  if (d > D2D_NORM_MAX_D) return PyLong_FromLong(D2D_ERR_UNSUPPORTED);
+  const at::Tensor w = param_of(wt, "weight", d, xt.scalar_type(), &pt);
+  const at::Tensor b = param_of(bt, "bias", d, xt.scalar_type(), &pt);
+  if (d > D2D_NORM_MAX_D) return D2D_ERR_UNSUPPORTED;
   On on(xt);
   const Rows x = rows_of(xt);
-  at::Tensor y = at::detail::empty_cuda(xt.sizes(), xt.options()), mean, rstd;
+  *y = at::detail::empty_cuda(xt.sizes(), xt.options());
   if (stats) {
     const auto f32 = xt.options().dtype(at::kFloat);
-    if (kind == D2D_NORM_LAYER) mean = at::detail::empty_cuda({x.n}, f32);
-    rstd = at::detail::empty_cuda({x.n}, f32);
+    if (h.kind == D2D_NORM_LAYER) *mean = at::detail::empty_cuda({x.n}, f32);
+    *rstd = at::detail::empty_cuda({x.n}, f32);
   }
-  const int rc = x.n == 0 ? D2D_OK
-                          : d2d_layer_norm(x.t.data_ptr(), x.stride, data_or_null(&w), data_or_null(&b), (float)eps,
-                                           kind, (float)offset, y.data_ptr(), (float*)data_or_null(&mean),
-                                           (float*)data_or_null(&rstd), x.n, (int)d, dt, param_code(pt, dt), on.stream);
-  if (rc != D2D_OK) return PyLong_FromLong(rc);
-  return wrap_all({y, mean, rstd});
-  END_HANDLE_TH_ERRORS
+  return d2d_layer_norm(address(x.t), x.stride, data_or_null(&w), data_or_null(&b), (float)h.eps, h.kind,
+                        (float)h.offset, address(*y), x.n ? (float*)data_or_null(mean) : nullptr,
+                        x.n ? (float*)data_or_null(rstd) : nullptr, x.n, (int)d, dt, param_code(pt, dt), on.stream);
 }
 
-// layer_norm_backward(dy, x, weight | None, mean | None, rstd, kind, weight offset, dx, dweight, dbias wanted)
-//   -> (dx, dweight, dbias), None where not wanted; without a weight the gradients are of x's dtype
-PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 10, "layer_norm_backward takes 10 arguments");
-  const at::Tensor& xt = needed(a[1], "x");
-  const at::Tensor& gt = needed(a[0], "dy", &xt);
+int norm_backward(const at::Tensor& gt, const at::Tensor& xt, const at::Tensor* wt, const at::Tensor* mean,
+                  const at::Tensor& rstd, const NormHow& h, const bool (&want)[3], at::Tensor* dx, at::Tensor* dw,
+                  at::Tensor* db) {
   const int dt = dtype_of(xt);
   of_type(gt, xt.scalar_type(), "dy");
   TORCH_CHECK_VALUE(xt.dim() >= 1 && xt.size(-1) > 0, "x must have rows of one value or more");
   TORCH_CHECK_VALUE(gt.sizes() == xt.sizes(), "dy must have the shape of x");
   const int64_t d = xt.size(-1);
   at::ScalarType pt = at::ScalarType::Undefined;
-  const at::Tensor w = param_of(given(a[2], "weight", &xt), "weight", d, xt.scalar_type(), &pt);
-  const at::Tensor* mean = given(a[3], "mean", &xt);
-  const at::Tensor& rstd = needed(a[4], "rstd", &xt);
-  const int kind = (int)PyLong_AsLong(a[5]);
-  const double offset = PyFloat_AsDouble(a[6]);
-  const int want[3] = {PyObject_IsTrue(a[7]), PyObject_IsTrue(a[8]), PyObject_IsTrue(a[9])};
-  if (PyErr_Occurred()) return nullptr;
-  if (d > D2D_NORM_MAX_D) return PyLong_FromLong(D2D_ERR_UNSUPPORTED);
+  const at::Tensor w = param_of(wt, "weight", d, xt.scalar_type(), &pt);
+  if (d > D2D_NORM_MAX_D) return D2D_ERR_UNSUPPORTED;
   On on(xt);
   const Rows x = rows_of(xt), g = rows_of(gt);
   for (const at::Tensor* t : {mean, &rstd})
@@ -673,49 +665,38 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       of_type(*t, at::kFloat, "statistics");
       TORCH_CHECK_VALUE(t->numel() == x.n && t->is_contiguous(), "mean and rstd must be contiguous, one value a row");
     }
-  TORCH_CHECK_VALUE(kind != D2D_NORM_LAYER || mean, "mean is missing");
+  TORCH_CHECK_VALUE(h.kind != D2D_NORM_LAYER || mean, "mean is missing");
   const auto po = xt.options().dtype(pt == at::ScalarType::Undefined ? xt.scalar_type() : pt);
-  at::Tensor dx, dw, db, ws;
-  if (want[0]) dx = at::detail::empty_cuda(xt.sizes(), xt.options());
-  if (want[1]) dw = at::detail::empty_cuda({d}, po);
-  if (want[2]) db = at::detail::empty_cuda({d}, po);
+  if (want[0]) *dx = at::detail::empty_cuda(xt.sizes(), xt.options());
+  if (want[1]) *dw = at::detail::empty_cuda({d}, po);
+  if (want[2]) *db = at::detail::empty_cuda({d}, po);
+  at::Tensor ws;
   size_t bytes = 0;
   if (want[1] || want[2]) {
     const int rc = d2d_layer_norm_workspace_bytes(x.n, (int)d, &bytes);
-    if (rc != D2D_OK) return PyLong_FromLong(rc);
+    if (rc != D2D_OK) return rc;
     ws = at::detail::empty_cuda({(int64_t)std::max<size_t>(bytes, 16)}, xt.options().dtype(at::kByte));
   }
-  // (tensors without rows have no address)
-  static float none;
-  const auto at_least = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : (void*)&none; };
-  const int rc = d2d_layer_norm_backward(
-      at_least(g.t), g.stride, at_least(x.t), x.stride, data_or_null(&w), kind, (float)offset,
-      mean ? (const float*)at_least(*mean) : nullptr, (const float*)at_least(rstd), x.n ? data_or_null(&dx) : nullptr,
-      data_or_null(&dw), data_or_null(&db), x.n, (int)d, dt, param_code(pt, dt), data_or_null(&ws), bytes, on.stream);
-  if (rc != D2D_OK) return PyLong_FromLong(rc);
-  return wrap_all({dx, dw, db});
-  END_HANDLE_TH_ERRORS
+  return d2d_layer_norm_backward(address(g.t), g.stride, address(x.t), x.stride, data_or_null(&w), h.kind,
+                                 (float)h.offset, mean ? (const float*)address(*mean) : nullptr,
+                                 (const float*)address(rstd), x.n ? data_or_null(dx) : nullptr, data_or_null(dw),
+                                 data_or_null(db), x.n, (int)d, dt, param_code(pt, dt), data_or_null(&ws), bytes,
+                                 on.stream);
 }
 
-// route(logits [N, E], k, scores, bias | None, groups, top_groups, renormalise, scale, mask bits | None, dense wanted)
-//   -> (weights, experts, routing tensor | None)
-PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 10, "route takes 10 arguments");
-  const at::Tensor& lt = needed(a[0], "logits");
+struct RouteHow {
+  int64_t k, scores, groups, top;
+  bool renormalise;
+  double scale;
+};
+
+int route_forward(const at::Tensor& lt, const at::Tensor* bt, const RouteHow& h, const at::Tensor* mask, bool dense,
+                  at::Tensor* w, at::Tensor* e, at::Tensor* rt) {
   const int dt = dtype_of(lt);
   TORCH_CHECK_VALUE(lt.dim() >= 1 && lt.size(-1) > 0, "logits must have one expert or more");
   const int64_t E = lt.size(-1), N = lt.numel() / E;
-  const int64_t k = PyLong_AsLong(a[1]), scores = PyLong_AsLong(a[2]);
-  const at::Tensor* bt = given(a[3], "bias", &lt);
-  const int64_t groups = PyLong_AsLong(a[4]), top = PyLong_AsLong(a[5]);
-  const int renorm = PyObject_IsTrue(a[6]);
-  const double scale = PyFloat_AsDouble(a[7]);
-  const at::Tensor* mask = given(a[8], "mask bits", &lt);
-  const int dense = PyObject_IsTrue(a[9]);
-  if (PyErr_Occurred()) return nullptr;
-  if (E > (1 << 20) || k < 0 || k > E || groups < 0 || groups > E || top < 0 || top > E)
-    return PyLong_FromLong(E > (1 << 20) ? D2D_ERR_UNSUPPORTED : D2D_ERR_BAD_ARG);
+  if (E > (1 << 20)) return D2D_ERR_UNSUPPORTED;
+  if (h.k < 0 || h.k > E || h.groups < 0 || h.groups > E || h.top < 0 || h.top > E) return D2D_ERR_BAD_ARG;
   On on(lt);
   at::Tensor bias;
   if (bt) {
@@ -728,28 +709,17 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       "mask bits: room for [tokens, ceil(experts / 32)] words");
   const at::Tensor logits = lt.contiguous();
   c10::SmallVector<int64_t, 5> shape(lt.sizes().begin(), lt.sizes().end());
-  shape.back() = k;
-  at::Tensor w = at::detail::empty_cuda(shape, lt.options().dtype(at::kFloat));
-  at::Tensor e = at::detail::empty_cuda(shape, lt.options().dtype(at::kInt)), rt;
-  if (dense) rt = at::detail::empty_cuda(lt.sizes(), lt.options());
-  static int none;                       // (tensors without tokens have no address; arguments are checked all the same)
-  const int rc = d2d_route(N ? logits.data_ptr() : &none, (const float*)data_or_null(&bias), (int)scores, (int)k, (int)groups,
-                           (int)top, renorm, (float)scale, N ? (int32_t*)e.data_ptr() : &none,
-                           N ? (float*)w.data_ptr() : (float*)&none, (uint32_t*)data_or_null(mask), data_or_null(&rt), N,
-                           (int)E, dt, on.stream);
-  if (rc != D2D_OK) return PyLong_FromLong(rc);
-  return wrap_all({w, e, rt});
-  END_HANDLE_TH_ERRORS
+  shape.back() = h.k;
+  *w = at::detail::empty_cuda(shape, lt.options().dtype(at::kFloat));
+  *e = at::detail::empty_cuda(shape, lt.options().dtype(at::kInt));
+  if (dense) *rt = at::detail::empty_cuda(lt.sizes(), lt.options());
+  return d2d_route(address(logits), (const float*)data_or_null(&bias), (int)h.scores, (int)h.k, (int)h.groups,
+                   (int)h.top, h.renormalise, (float)h.scale, (int32_t*)address(*e), (float*)address(*w),
+                   (uint32_t*)data_or_null(mask), data_or_null(rt), N, (int)E, dt, on.stream);
 }
 
-// route_backward(dweights, logits, experts, weights, scores, renormalise, scale) -> dlogits
-PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 7, "route_backward takes 7 arguments");
-  const at::Tensor& lt = needed(a[1], "logits");
-  const at::Tensor& gt = needed(a[0], "dweights", &lt);
-  const at::Tensor& et = needed(a[2], "experts", &lt);
-  const at::Tensor& wt = needed(a[3], "weights", &lt);
+int route_gradient(const at::Tensor& gt, const at::Tensor& lt, const at::Tensor& et, const at::Tensor& wt,
+                   const RouteHow& h, at::Tensor* out) {
   const int dt = dtype_of(lt);
   of_type(gt, at::kFloat, "dweights");
   of_type(wt, at::kFloat, "weights");
@@ -760,19 +730,202 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                         wt.sizes() == et.sizes() && gt.sizes() == et.sizes(),
                     "experts, weights and dweights must be [.., k] for logits [.., experts]");
   const int64_t k = et.size(-1);
-  const int64_t scores = PyLong_AsLong(a[4]);
-  const int renorm = PyObject_IsTrue(a[5]);
-  const double scale = PyFloat_AsDouble(a[6]);
-  if (PyErr_Occurred()) return nullptr;
-  if (E > (1 << 20) || k > E) return PyLong_FromLong(k > E ? D2D_ERR_BAD_ARG : D2D_ERR_UNSUPPORTED);
+  if (E > (1 << 20) || k > E) return k > E ? D2D_ERR_BAD_ARG : D2D_ERR_UNSUPPORTED;
   On on(lt);
   const at::Tensor logits = lt.contiguous(), e = et.contiguous(), w = wt.contiguous(), g = gt.contiguous();
-  at::Tensor out = at::detail::empty_cuda(lt.sizes(), lt.options());
-  static int none;
-  const auto at_least = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : (void*)&none; };
-  const int rc = d2d_route_backward(at_least(logits), (const int32_t*)at_least(e), (const float*)at_least(w),
-                                    (const float*)at_least(g), (int)scores, renorm, (float)scale, at_least(out), N,
-                                    (int)E, (int)k, dt, on.stream);
+  *out = at::detail::empty_cuda(lt.sizes(), lt.options());
+  return d2d_route_backward(address(logits), (const int32_t*)address(e), (const float*)address(w),
+                            (const float*)address(g), (int)h.scores, h.renormalise, (float)h.scale, address(*out), N,
+                            (int)E, (int)k, dt, on.stream);
+}
+
+// ---- the same under autograd ----------------------------------------------------------
+// First derivatives only: where the gradients' own graph is asked for, differentiating it says so.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+variable_list once(variable_list grads, const variable_list& incoming, const char* what) {
+  bool twice = at::GradMode::is_enabled(), any = false;
+  for (const at::Tensor& g : incoming) any |= g.defined() && g.requires_grad();
+  if (!twice || !any) return grads;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has first derivatives only",
+                                                               (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& w,
+                            const std::optional<at::Tensor>& b, const NormHow& h) {
+    at::Tensor y, mean, rstd;
+    const int rc = norm_forward(x, w ? &*w : nullptr, b ? &*b : nullptr, h, true, &y, &mean, &rstd);
+    TORCH_CHECK(rc == D2D_OK, "d2d_layer_norm: ", d2d_strerror(rc));
+    ctx->save_for_backward({x, w ? *w : at::Tensor(), mean, rstd});
+    ctx->saved_data["how"] = std::vector<double>{h.eps, h.offset, (double)h.kind, b ? 1.0 : 0.0};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const auto how = ctx->saved_data["how"].toDoubleVector();
+    const NormHow h = {how[0], how[1], (int)how[2]};
+    const bool weight = s[1].defined(), bias = how[3] != 0.0;      // (only tensors that are there are counted)
+    const bool want[3] = {ctx->needs_input_grad(0), weight && ctx->needs_input_grad(1),
+                          bias && ctx->needs_input_grad(weight ? 2 : 1)};
+    variable_list out(4);
+    if (!g[0].defined()) return out;
+    const int rc = norm_backward(g[0], s[0], s[1].defined() ? &s[1] : nullptr, s[2].defined() ? &s[2] : nullptr, s[3], h,
+                                 want, &out[0], &out[1], &out[2]);
+    TORCH_CHECK(rc == D2D_OK, "d2d_layer_norm_backward: ", d2d_strerror(rc));
+    return once(std::move(out), g, "layer_norm");
+  }
+};
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const std::optional<at::Tensor>& bias,
+                               const RouteHow& h) {
+    at::Tensor w, e, rt;
+    const int rc = route_forward(logits, bias ? &*bias : nullptr, h, nullptr, false, &w, &e, &rt);
+    TORCH_CHECK(rc == D2D_OK, "d2d_route: ", d2d_strerror(rc));
+    ctx->save_for_backward({logits, e, w});
+    ctx->mark_non_differentiable({e});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["scores"] = h.scores;
+    ctx->saved_data["renormalise"] = h.renormalise;
+    ctx->saved_data["scale"] = h.scale;
+    return {w, e};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(3);
+    if (!g[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    RouteHow h = {};
+    h.scores = ctx->saved_data["scores"].toInt();
+    h.renormalise = ctx->saved_data["renormalise"].toBool();
+    h.scale = ctx->saved_data["scale"].toDouble();
+    const int rc = route_gradient(g[0], s[0], s[1], s[2], h, &out[0]);
+    TORCH_CHECK(rc == D2D_OK, "d2d_route_backward: ", d2d_strerror(rc));
+    return once(std::move(out), g, "route_tokens");
+  }
+};
+
+std::optional<at::Tensor> optional(const at::Tensor* t) { return t ? std::optional<at::Tensor>(*t) : std::nullopt; }
+
+// ---- calls from Python ------------------------------------------------------------------
+// layer_norm(x, weight | None, bias | None, eps, kind, weight offset, statistics wanted) -> (y, mean | None, rstd | None)
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "layer_norm takes 7 arguments");
+  const at::Tensor& x = needed(a[0], "x");
+  const at::Tensor *w = given(a[1], "weight", &x), *b = given(a[2], "bias", &x);
+  NormHow h = {PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[5]), (int)PyLong_AsLong(a[4])};
+  const int stats = PyObject_IsTrue(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor y, mean, rstd;
+  const int rc = norm_forward(x, w, b, h, stats, &y, &mean, &rstd);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({y, mean, rstd});
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_autograd(x, weight | None, bias | None, eps, kind, weight offset) -> y
+PyObject* layer_norm_autograd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 6, "layer_norm_autograd takes 6 arguments");
+  const at::Tensor& x = needed(a[0], "x");
+  const at::Tensor *w = given(a[1], "weight", &x), *b = given(a[2], "bias", &x);
+  NormHow h = {PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[5]), (int)PyLong_AsLong(a[4])};
+  if (PyErr_Occurred()) return nullptr;
+  // refusals by status code come before autograd
+  if (x.dim() >= 1 && x.size(-1) > D2D_NORM_MAX_D) return PyLong_FromLong(D2D_ERR_UNSUPPORTED);
+  if (!(h.eps >= 0.0)) return PyLong_FromLong(D2D_ERR_BAD_ARG);
+  return wrap(NormFunction::apply(x, optional(w), optional(b), h));
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_backward(dy, x, weight | None, mean | None, rstd, kind, weight offset, dx, dweight, dbias wanted)
+//   -> (dx, dweight, dbias), None where not wanted; without a weight the gradients are of x's dtype
+PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "layer_norm_backward takes 10 arguments");
+  const at::Tensor& x = needed(a[1], "x");
+  const at::Tensor& g = needed(a[0], "dy", &x);
+  const at::Tensor *w = given(a[2], "weight", &x), *mean = given(a[3], "mean", &x);
+  const at::Tensor& rstd = needed(a[4], "rstd", &x);
+  NormHow h = {0.0, PyFloat_AsDouble(a[6]), (int)PyLong_AsLong(a[5])};
+  const bool want[3] = {PyObject_IsTrue(a[7]) == 1, PyObject_IsTrue(a[8]) == 1, PyObject_IsTrue(a[9]) == 1};
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor dx, dw, db;
+  const int rc = norm_backward(g, x, w, mean, rstd, h, want, &dx, &dw, &db);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({dx, dw, db});
+  END_HANDLE_TH_ERRORS
+}
+
+// from a[1] on: k, scores, bias | None, groups, top_groups, renormalise, scale
+bool route_how(PyObject* const* a, const at::Tensor& logits, RouteHow* h, const at::Tensor** bias) {
+  *bias = given(a[3], "bias", &logits);
+  *h = {PyLong_AsLong(a[1]), PyLong_AsLong(a[2]),           PyLong_AsLong(a[4]),
+        PyLong_AsLong(a[5]), PyObject_IsTrue(a[6]) == 1, PyFloat_AsDouble(a[7])};
+  return !PyErr_Occurred();
+}
+
+// route(logits [.., E], k, scores, bias | None, groups, top_groups, renormalise, scale, mask bits | None, dense wanted)
+//   -> (weights, experts, routing tensor | None)
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "route takes 10 arguments");
+  const at::Tensor& logits = needed(a[0], "logits");
+  RouteHow h;
+  const at::Tensor* bias;
+  if (!route_how(a, logits, &h, &bias)) return nullptr;
+  const at::Tensor* mask = given(a[8], "mask bits", &logits);
+  const int dense = PyObject_IsTrue(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor w, e, rt;
+  const int rc = route_forward(logits, bias, h, mask, dense, &w, &e, &rt);
+  if (rc != D2D_OK) return PyLong_FromLong(rc);
+  return wrap_all({w, e, rt});
+  END_HANDLE_TH_ERRORS
+}
+
+// route_autograd(logits, k, scores, bias | None, groups, top_groups, renormalise, scale) -> (weights, experts)
+PyObject* route_autograd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 8, "route_autograd takes 8 arguments");
+  const at::Tensor& logits = needed(a[0], "logits");
+  RouteHow h;
+  const at::Tensor* bias;
+  if (!route_how(a, logits, &h, &bias)) return nullptr;
+  // refusals by status code come before autograd: the same call for no tokens
+  if (logits.dim() >= 1 && logits.size(-1) > 0) {
+    int none = 0;
+    const auto small = [](int64_t v) { return (int)std::min<int64_t>(std::max<int64_t>(v, -1), 1 << 21); };
+    const int rc = d2d_route(&none, nullptr, (int)h.scores, small(h.k), small(h.groups), small(h.top), h.renormalise,
+                             (float)h.scale, &none, (float*)&none, nullptr, nullptr, 0, small(logits.size(-1)),
+                             dtype_of(logits), nullptr);
+    if (rc != D2D_OK) return PyLong_FromLong(rc);
+  }
+  const variable_list r = RouteFunction::apply(logits, optional(bias), h);
+  return wrap_all({r[0], r[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// route_backward(dweights, logits, experts, weights, scores, renormalise, scale) -> dlogits
+PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "route_backward takes 7 arguments");
+  const at::Tensor& logits = needed(a[1], "logits");
+  const at::Tensor& g = needed(a[0], "dweights", &logits);
+  const at::Tensor& e = needed(a[2], "experts", &logits);
+  const at::Tensor& w = needed(a[3], "weights", &logits);
+  RouteHow h = {};
+  h.scores = PyLong_AsLong(a[4]);
+  h.renormalise = PyObject_IsTrue(a[5]) == 1;
+  h.scale = PyFloat_AsDouble(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor out;
+  const int rc = route_gradient(g, logits, e, w, h, &out);
   if (rc != D2D_OK) return PyLong_FromLong(rc);
   return wrap(out);
   END_HANDLE_TH_ERRORS
@@ -893,6 +1046,8 @@ PyObject* run_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef kMethods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
+    {"layer_norm_autograd", (PyCFunction)(void (*)(void))layer_norm_autograd, METH_FASTCALL, nullptr},
+    {"route_autograd", (PyCFunction)(void (*)(void))route_autograd, METH_FASTCALL, nullptr},
     {"layer_norm_backward", (PyCFunction)(void (*)(void))layer_norm_backward, METH_FASTCALL, nullptr},
     {"route", (PyCFunction)(void (*)(void))route, METH_FASTCALL, nullptr},
     {"route_backward", (PyCFunction)(void (*)(void))route_backward, METH_FASTCALL, nullptr},

@@ -166,6 +166,45 @@ def test_norm_gradient_against_differences():
 
 
 @pytest.mark.gpu
+def test_gradients_of_some_inputs_only():
+    """What autograd does not ask for is left out; a second derivative is refused, not wrong."""
+    import d2dmoe_b200 as D
+    x, w, b, dy = norm_inputs(50, 96, "fp32", "same", "layer", 0)
+    y, mean, rstd = D.ops.layer_norm(x, w, b)
+    want = D.ops.layer_norm_backward(dy, x, w, mean, rstd)
+    for mask in range(1, 8):
+        ins = [t.detach().clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        D.layer_norm(*ins).backward(dy)
+        for i, t in enumerate(ins):
+            assert (t.grad is None) == (not mask >> i & 1)
+            assert t.grad is None or torch.equal(t.grad, want[i])
+    # a bias without a weight
+    bb = b.detach().clone().requires_grad_()
+    D.layer_norm(x, None, bb).backward(dy)
+    within(bb.grad, dy.double().sum(0), 128 * U * dy.double().abs().sum(0), "bias alone")
+    leaf = x.detach().clone().requires_grad_()
+    g = torch.autograd.grad(D.layer_norm(leaf, w, b), leaf, dy.clone().requires_grad_(), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        g.sum().backward()
+    leaf = x.detach().clone().requires_grad_()
+    wt, e = D.route_tokens(leaf, 3)
+    assert wt.requires_grad and not e.requires_grad
+    g = torch.autograd.grad(wt, leaf, torch.ones_like(wt).requires_grad_(), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        g.sum().backward()
+    with torch.no_grad():
+        assert not D.layer_norm(leaf).requires_grad and not D.route_tokens(leaf, 3)[0].requires_grad
+    for call in (lambda: D.layer_norm(leaf, eps=-1.0), lambda: D.route_tokens(leaf, 200),
+                 lambda: D.route_tokens(leaf, 2, groups=5), lambda: D.route_tokens(leaf, 2, scale=-1.0)):
+        with pytest.raises(D.ops._capi.D2DError):
+            call()
+    with pytest.raises(TypeError):
+        D.layer_norm(leaf, w.bfloat16())
+    with pytest.raises(ValueError):
+        D.route_tokens(leaf, 2, bias=w[:3])
+
+
+@pytest.mark.gpu
 def test_norm_shapes_and_odd_values():
     import d2dmoe_b200 as D
     g = gen(3)
