@@ -664,7 +664,7 @@ struct BackwardArgs {
 };
 
 template <typename T, int V, int L, int EL>
-__global__ void __launch_bounds__(NT) route_backward_kernel(BackwardArgs a) {
+__global__ void __launch_bounds__(NT, EL == 16 ? 8 : 4) route_backward_kernel(BackwardArgs a) {
   extern __shared__ __align__(16) double scratch[];
   constexpr int TOKENS = 32 / L;
   grid_launch_dependents();
@@ -685,26 +685,41 @@ __global__ void __launch_bounds__(NT) route_backward_kernel(BackwardArgs a) {
     T* const to = reinterpret_cast<T*>(a.dlogits) + t * E;
     Row<T, V, L, EL> row;
     if (all) row.load(l, E, q, in);
+    // a lane's slots: the first stays in registers, the others (k > L) are read again
+    struct Slot {
+      int e;
+      float g, p;
+    };
+    auto slot = [&](int j) {
+      Slot v = {in && j < a.k ? a.experts[t * a.k + j] : -1, 0.f, 0.f};
+      if ((unsigned)v.e >= (unsigned)E) {
+        v.e = -1;
+      } else {
+        v.g = a.scale * a.dweights[t * a.k + j];
+        v.p = a.weights[t * a.k + j] * inv;
+      }
+      return v;
+    };
+    const Slot mine0 = slot(q);
     float dot = 0.f;
-    bool any = false;
+    bool any = mine0.e >= 0;
     if (a.renormalise || a.softmax) {
-      for (int j = q; j < a.k; j += L) {
-        const int e = in ? a.experts[t * a.k + j] : -1;
-        if ((unsigned)e < (unsigned)E) {
-          any = true;
-          dot = fmaf(a.weights[t * a.k + j] * inv, a.scale * a.dweights[t * a.k + j], dot);
-        }
+      dot = mine0.p * mine0.g;
+      for (int j = q + L; j < a.k; j += L) {
+        const Slot v = slot(j);
+        any |= v.e >= 0;
+        dot = fmaf(v.p, v.g, dot);
       }
       dot = sum_lanes<L>(dot);
     }
-    for (int j = q; j < a.k; j += L) {
-      const int e = in ? a.experts[t * a.k + j] : -1;
-      if ((unsigned)e >= (unsigned)E) continue;
-      const float g = a.scale * a.dweights[t * a.k + j], p = a.weights[t * a.k + j] * inv;
-      float d = a.renormalise ? p * (g - dot) : all ? g : p * g;
-      if (!a.softmax) d *= 1.f / (1.f + expf(DT<T>::to_f(l[e])));            // 1 - sigmoid
-      atomicAdd(&share[e], d);             // (an expert that is there twice has both shares)
-    }
+    auto put = [&](const Slot& v) {
+      if (v.e < 0) return;
+      float d = a.renormalise ? v.p * (v.g - dot) : all ? v.g : v.p * v.g;
+      if (!a.softmax) d *= 1.f / (1.f + expf(DT<T>::to_f(l[v.e])));          // 1 - sigmoid
+      atomicAdd(&share[v.e], d);           // (an expert that is there twice has both shares)
+    };
+    put(mine0);
+    for (int j = q + L; j < a.k; j += L) put(slot(j));
     __syncwarp();
     if (all) {
       const float m = max_lanes<L>(row.largest());
@@ -719,11 +734,17 @@ __global__ void __launch_bounds__(NT) route_backward_kernel(BackwardArgs a) {
         const int e = (v * L + q) * V;
         if (!in || e >= E) continue;
         float d[V];
+        if constexpr (V == 1) {
+          d[0] = share[e];
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          d[i] = chosen ? s[v * V + i] * is * (share[e + i] - dot) : 0.f;
-          share[e + i] = 0.f;
+          for (int i = 0; i < V / 4; ++i) {
+            const float4 x = *(reinterpret_cast<const float4*>(share + e) + i);
+            d[4 * i] = x.x, d[4 * i + 1] = x.y, d[4 * i + 2] = x.z, d[4 * i + 3] = x.w;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] = chosen ? s[v * V + i] * is * (d[i] - dot) : 0.f;
         if constexpr (V == 1) to[e] = DT<T>::from_f(d[0]);
         else if constexpr (V == 4) *reinterpret_cast<float4*>(to + e) = make_float4(d[0], d[1], d[2], d[3]);
         else
@@ -731,28 +752,27 @@ __global__ void __launch_bounds__(NT) route_backward_kernel(BackwardArgs a) {
                                                          pack_bf16x2(d[4], d[5]), pack_bf16x2(d[6], d[7]));
       }
     } else {
-      for (int e = q * V; e < E; e += L * V) {
+      for (int e = q * V; e < E && in; e += L * V) {
         if constexpr (V == 1) {
-          if (in) to[e] = DT<T>::from_f(share[e]);
-          share[e] = 0.f;
+          to[e] = DT<T>::from_f(share[e]);
         } else {
           float4 d[V / 4];
 #pragma unroll
-          for (int i = 0; i < V / 4; ++i) {
-            float4* const at = reinterpret_cast<float4*>(share + e) + i;
-            d[i] = *at;
-            *at = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-          if constexpr (V == 4) {
-            if (in) *reinterpret_cast<float4*>(to + e) = d[0];
-          } else {
-            if (in)
-              *reinterpret_cast<uint4*>(to + e) =
-                  make_uint4(pack_bf16x2(d[0].x, d[0].y), pack_bf16x2(d[0].z, d[0].w),
-                             pack_bf16x2(d[1].x, d[1].y), pack_bf16x2(d[1].z, d[1].w));
-          }
+          for (int i = 0; i < V / 4; ++i) d[i] = *(reinterpret_cast<const float4*>(share + e) + i);
+          if constexpr (V == 4)
+            *reinterpret_cast<float4*>(to + e) = d[0];
+          else
+            *reinterpret_cast<uint4*>(to + e) = make_uint4(pack_bf16x2(d[0].x, d[0].y), pack_bf16x2(d[0].z, d[0].w),
+                                                           pack_bf16x2(d[1].x, d[1].y), pack_bf16x2(d[1].z, d[1].w));
         }
       }
+    }
+    __syncwarp();
+    // back to zero, where something was
+    if (mine0.e >= 0) share[mine0.e] = 0.f;
+    for (int j = q + L; j < a.k; j += L) {
+      const int e = slot(j).e;
+      if (e >= 0) share[e] = 0.f;
     }
     __syncwarp();
   }
@@ -776,11 +796,14 @@ int launch_shape(RouteArgs a, int sms, cudaStream_t s) {
   return launch_pdl(k, dim3((unsigned)route_grid(ceil_div64(a.N, WARPS * TOKENS), sms, 16)), dim3(NT), smem, s, a);
 }
 
-// Lists of 8 or 16 keys.  Rows that allow no vectors take the widest forms only.
+// Lists of 4, 8 or 16 keys (4 of 96, 65536 tokens: lists of 8 take TIME8 us, lists of 4 TIME4).  Rows that allow no vectors
+// take the widest forms only.
 template <typename T, int V, int L, int EL, int MODE>
 int launch_list(const RouteArgs& a, int sms, cudaStream_t s) {
-  if constexpr (V > 1)
+  if constexpr (V > 1) {
+    if (a.k <= 4) return launch_shape<T, V, L, EL, 4, MODE>(a, sms, s);
     if (a.k <= 8) return launch_shape<T, V, L, EL, 8, MODE>(a, sms, s);
+  }
   if constexpr (EL >= 16) return launch_shape<T, V, L, EL, 16, MODE>(a, sms, s);
   return D2D_ERR_UNSUPPORTED;
 }
