@@ -1257,7 +1257,7 @@ int launch_experts_umma_pairs(const void* x, int32_t* pairs, int32_t* offsets, c
   p.H = H;
   p.act = act;
   p.packed = (const uint8_t*)packed;
-  p.g = experts_geo(d, H, glu, N * k);     // (a token may want an expert twice)
+  p.g = experts_geo(d, H, glu, N);         // (longer lists, of tokens that want an expert twice, are cut into more tiles)
   p.token_idx = pairs;
   p.offsets = offsets;
   p.warm = true;

@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ?
           worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
           other = fmaxf(other, __shfl_xor_sync(0xffffffffu, other, o));
         }
-        // (two scores and their sum: twice the bound below)
-        unsure = other > -INFINITY && worst - other <= 8e-6f + 1e-6f * fabsf(worst);
+        // (two scores and their sum: twice the bound of single ones, below)
+        unsure = other > -INFINITY && worst - other <= 1.2e-5f + 1e-6f * fabsf(worst);
 #pragma unroll
         for (int v = 0; v < EL / V; ++v) {
           const int e = (v * L + q) * V;
@@ -537,13 +537,14 @@ __global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ?
         }
       }
       if (a.bias) {
-        // Scores of the fast exponential and reciprocal are off by less than 6e-7 (softmax: 2 ulp of the exponential,
-        // as much of the sum; sigmoid: less), their sums with the bias by half an ulp more: two
-        // of them in the wrong order differ by less than 2e-6 + 2^-23 |c|.  Keys take the range of 4 below
-        // the largest c in steps of 2^(2 + index bits - 32); what lies lower has the lowest key.
+        // How far two c in the wrong order can be apart: the exponentials and reciprocals of each are off by 3e-7 at most, a
+        // softmax's sum (37 roundings, the same for all) by 2.2e-6 of the difference of two scores, the
+        // sums with the bias by half an ulp, 6e-8 (4 + |largest c|) each, the keys' own rounding by 2.4e-7 each: less than
+        // 5e-6 + 1.2e-7 |largest c|.  Keys take the range of 4 below the largest c in steps of
+        // 2^(2 + index bits - 32); what lies lower has the lowest key.
         const float scale = (float)(1u << (30 - index_bits)), zero = (4.f - top) * scale;
         const uint32_t most = 0xffffffffu >> index_bits;
-        near = (uint32_t)fminf((4e-6f + 5e-7f * fabsf(top)) * scale, 1e9f) + 2u;
+        near = (uint32_t)fminf((6e-6f + 5e-7f * fabsf(top)) * scale, 1e9f) + 2u;
         least = 1u << index_bits;
 #pragma unroll
         for (int i = 0; i < EL; ++i) {
@@ -796,8 +797,8 @@ int launch_shape(RouteArgs a, int sms, cudaStream_t s) {
   return launch_pdl(k, dim3((unsigned)route_grid(ceil_div64(a.N, WARPS * TOKENS), sms, 16)), dim3(NT), smem, s, a);
 }
 
-// Lists of 4, 8 or 16 keys (4 of 96, 65536 tokens: lists of 8 take TIME8 us, lists of 4 TIME4).  Rows that allow no vectors
-// take the widest forms only.
+// Lists of 4, 8 or 16 keys (4 of 96, 65536 tokens: lists of 8 take 23 us, lists of 4 20).  Rows that allow no vectors take the
+// widest forms only.
 template <typename T, int V, int L, int EL, int MODE>
 int launch_list(const RouteArgs& a, int sms, cudaStream_t s) {
   if constexpr (V > 1) {
@@ -807,7 +808,8 @@ int launch_list(const RouteArgs& a, int sms, cudaStream_t s) {
   if constexpr (EL >= 16) return launch_shape<T, V, L, EL, 16, MODE>(a, sms, s);
   return D2D_ERR_UNSUPPORTED;
 }
-// Lanes per token: 32 logits a lane where their order is all (fewer merges), 16 where the scores need registers too.
+// Lanes per token: 32 logits a lane where their order is all (fewer merges), 16 where the scores need registers too (16384 x 256
+// with groups: 32 take 28 us, 16 take 30).
 template <typename T, int V, int MODE>
 int launch_lanes(const RouteArgs& a, int sms, cudaStream_t s) {
   if constexpr (V > 1) {
@@ -818,7 +820,7 @@ int launch_lanes(const RouteArgs& a, int sms, cudaStream_t s) {
       if (a.E <= 256) return launch_list<T, V, 8, 32, MODE>(a, sms, s);
     } else {
       if (a.E <= 128) return launch_list<T, V, 8, 16, MODE>(a, sms, s);
-      if (a.E <= 256) return launch_list<T, V, 16, 16, MODE>(a, sms, s);
+      if (a.E <= 256) return launch_list<T, V, 8, 32, MODE>(a, sms, s);
     }
   } else {
     if (a.E <= 128) return launch_list<T, V, 8, 16, MODE>(a, sms, s);

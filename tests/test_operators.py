@@ -649,6 +649,52 @@ def test_weighted_experts_strided_and_misaligned():
                                                                      last_bias=lb))
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Buffers of more than 2^31 elements: rows at their ends against the references of those rows."""
+    import d2dmoe_b200 as D
+    g = gen(1)
+    d, N = 2048, 1_100_000
+    x = torch.empty(N, d, dtype=torch.bfloat16, device="cuda")
+    for part in x.split(1 << 17):
+        part.copy_(randn(g, *part.shape))
+    w = 1 + 0.1 * randn(g, d)
+    rows = torch.tensor([0, 1, 1_048_575, 1_048_576, N - 2, N - 1], device="cuda")
+    ref = norm_reference(x[rows], w, None, 1e-5, "layer", 0.0, x[rows])
+    y, mean, rstd = D.ops.layer_norm(x, w)
+    within(y[rows], *ref["y"], "y")
+    dx, dw, db = D.ops.layer_norm_backward(x, x, w, mean, rstd)
+    within(dx[rows], *ref["dx"], "dx")
+    # sum of x xh = sum of x^2 rstd - x mean rstd over the columns; N terms in blocks of a few thousand steps each
+    total = torch.zeros(d, dtype=torch.float64, device="cuda")
+    for i, part in enumerate(x.split(1 << 17)):
+        at = slice(i << 17, (i << 17) + part.shape[0])
+        total += (part.double() * (part.double() - mean[at, None]) * rstd[at, None]).sum(0)
+    assert ((dw - total).abs() <= 1e-4 * total.abs() + 1.0).all()
+    del x, y, dx
+    N, E, k = 131_072, 128, 8
+    x, e, wt, w1, b1, w2, up, lb = experts_case(N, 2048, E, 16, k, "bf16", False, False)
+    packed = D.ops.prepack_experts(w1, b1, w2)
+    out = D.ops.experts_weighted(x, e, wt, w1, b1, w2, "relu", packed=packed)
+    rows = torch.tensor([0, 1, 65_535, 131_000, N - 1], device="cuda")
+    within(out[rows], *experts_reference(x[rows], e[rows], wt[rows], w1, b1, w2, "relu"), "experts")
+    del out, x
+    N = 17_000_000
+    logits = torch.empty(N, E, dtype=torch.bfloat16, device="cuda")
+    for part in logits.split(1 << 20):
+        part.copy_(randn(g, *part.shape))
+    w, e, rt = D.ops.route(logits, 2, routing_tensor=True)
+    dl = D.ops.route_backward(torch.ones_like(w), logits, e, w, scores="sigmoid")
+    rows = torch.tensor([0, 16_777_215, 16_777_216, N - 1], device="cuda")
+    W, I, _ = route_reference(logits[rows], 2)
+    assert torch.equal(e[rows].cpu(), I)
+    within(w[rows].cpu(), W, 1e-5 * W, "weights")
+    assert torch.equal((rt[rows] > 0).nonzero()[:, 1].view(-1, 2).sort(1).values.cpu(), I.long().sort(1).values)
+    want = route_gradient(logits[rows], torch.ones(4, 2), e[rows], "sigmoid", True, 1.0)
+    # (the weights are softmax's here, any will do for the addresses: only where the gradient is not zero is compared)
+    assert torch.equal((dl[rows] != 0).cpu() | (want == 0), torch.ones(4, E, dtype=torch.bool))
+
+
 # -- together, as a layer runs them -----------------------------------------------------------------------
 def weighted_layer(dtype="bf16", glu=False, d=256, E=24, H=64, k=4, residual=False, seed=1, **routing):
     import d2dmoe_b200 as D
