@@ -41,7 +41,7 @@ __device__ __forceinline__ void add_row_norms(const float* part, float* rown, in
 // tokens the launch is one work item per SM and its duration is that item's).
 // PAIRS: the lists hold pairs p = token * slots + slot; out row p is stored, in fp32, and nothing is rounded.
 template <typename T, bool GLU, int TM_, bool PAIRS>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, PAIRS ? 2 : 1)
 experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_idx,
                     const int32_t* __restrict__ offsets, const T* __restrict__ w1,
                     const T* __restrict__ b1, const T* __restrict__ w_up,
@@ -158,11 +158,21 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
             xs[r * XP + k] =
                 (t >= 0 && kc + k < d) ? DT<T>::to_f(x[(int64_t)t * d + kc + k]) : 0.f;
           }
-          for (int i = tid; i < KC * CB; i += NT) {
-            const int k = i / CB, c = i % CB;
-            const bool ok = (kc + k < d) && (hc + c < H);
-            ws[k * WP + c] = ok ? DT<T>::to_f(w1e[(int64_t)(kc + k) * H + hc + c]) : 0.f;
-            if (GLU) wu[k * WP + c] = ok ? DT<T>::to_f(wue[(int64_t)(kc + k) * H + hc + c]) : 0.f;
+          if constexpr (PAIRS) {           // (only blocks of 32 columns that there are)
+            for (int c = lane; c < CB && hc + (c & ~31) < H; c += 32)
+#pragma unroll
+              for (int k = ty; k < KC; k += NT / 32) {
+                const bool ok = (kc + k < d) && (hc + c < H);
+                ws[k * WP + c] = ok ? DT<T>::to_f(w1e[(int64_t)(kc + k) * H + hc + c]) : 0.f;
+                if (GLU) wu[k * WP + c] = ok ? DT<T>::to_f(wue[(int64_t)(kc + k) * H + hc + c]) : 0.f;
+              }
+          } else {
+            for (int i = tid; i < KC * CB; i += NT) {
+              const int k = i / CB, c = i % CB;
+              const bool ok = (kc + k < d) && (hc + c < H);
+              ws[k * WP + c] = ok ? DT<T>::to_f(w1e[(int64_t)(kc + k) * H + hc + c]) : 0.f;
+              if (GLU) wu[k * WP + c] = ok ? DT<T>::to_f(wue[(int64_t)(kc + k) * H + hc + c]) : 0.f;
+            }
           }
         }
         __syncthreads();
@@ -199,6 +209,7 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
             }
           }
         };
+        if (PAIRS && hc + CW * cg >= H) continue;            // a warp without columns
         load_set(0, 0);
 #pragma unroll
         for (int k4 = 0; k4 < KC; k4 += 8) {
@@ -255,14 +266,24 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
             *reinterpret_cast<float4*>(&ws[(wk + 8 * j) * WP + wc]) = pw[j];
           if (kc + KC < H) prefetch2(kc + KC);
         } else {
-          for (int i = tid; i < KC * CB; i += NT) {
-            const int k = i / CB, c = i % CB;
-            ws[k * WP + c] = (kc + k < H && dc + c < d)
-                                 ? DT<T>::to_f(w2e[(int64_t)(kc + k) * d + dc + c])
-                                 : 0.f;
+          if constexpr (PAIRS) {
+            for (int c = lane; c < CB && dc + (c & ~31) < d; c += 32)
+#pragma unroll
+              for (int k = ty; k < KC; k += NT / 32)
+                ws[k * WP + c] = (kc + k < H && dc + c < d)
+                                     ? DT<T>::to_f(w2e[(int64_t)(kc + k) * d + dc + c])
+                                     : 0.f;
+          } else {
+            for (int i = tid; i < KC * CB; i += NT) {
+              const int k = i / CB, c = i % CB;
+              ws[k * WP + c] = (kc + k < H && dc + c < d)
+                                   ? DT<T>::to_f(w2e[(int64_t)(kc + k) * d + dc + c])
+                                   : 0.f;
+            }
           }
         }
         __syncthreads();
+        if (PAIRS && dc + CW * cg >= d) continue;
         const int kn = min(KC, H - kc);
         // four hidden columns per activation vector; two register sets as in the first product
         float4 ha[2][RPT], wv2[2][4];

@@ -60,6 +60,12 @@ struct Vec<bf16, 8> {
   }
 };
 
+// a load that stays behind the wait (its pointer need not be `fresh`, which would keep it in registers)
+__device__ __forceinline__ float load_in_order(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
 template <int V>
 __device__ __forceinline__ void store_vec(float* p, const float* f) {
   if (V == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
@@ -272,7 +278,8 @@ norm_forward_kernel(const T* __restrict__ x, const P* __restrict__ gamma, const 
   constexpr int NP = VPT * V / 2;
   grid_launch_dependents();
   grid_dependency_wait();
-  fresh(x, gamma, beta);
+  fresh(gamma, beta);
+  if (V == 1) fresh(x);                      // (vectors travel by cp.async, which the wait holds back)
   const int ti = threadIdx.x & (s.tpr - 1), slot = threadIdx.x / s.tpr, rows = blockDim.x / s.tpr;
   const int nv = s.d / V;
   const bool ragged = nv != s.tpr * VPT;
@@ -362,7 +369,8 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const P*
   constexpr int NP = VPT * V / 2;
   grid_launch_dependents();
   grid_dependency_wait();
-  fresh(dy, x, gamma, mean_in, rstd_in);
+  fresh(gamma);
+  if (V == 1) fresh(dy, x);
   const int ti = threadIdx.x & (s.tpr - 1), slot = threadIdx.x / s.tpr, rows = blockDim.x / s.tpr;
   const int nv = s.d / V;
   const int64_t step = (int64_t)gridDim.x * rows;
@@ -390,7 +398,8 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const P*
   if (COLS)
 #pragma unroll
     for (int k = 0; k < NP; ++k) dg[k] = db[k] = 0;
-  float mean = row < s.N && mean_in ? __ldg(mean_in + row) : 0.f, rstd = row < s.N ? __ldg(rstd_in + row) : 0.f;
+  float mean = row < s.N && mean_in ? load_in_order(mean_in + row) : 0.f,
+        rstd = row < s.N ? load_in_order(rstd_in + row) : 0.f;
   __syncthreads();
   for (int64_t first = (int64_t)blockIdx.x * rows; first < s.N; first += step, row += step) {
     const bool in = row < s.N, more = row + step < s.N;
@@ -402,8 +411,8 @@ norm_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const P*
       to_pairs(raw[1], g);
     }
     fetch(A::RING ? (ahead.stage + A::STAGES - 2) % A::STAGES : 0, row + A::DEPTH * step);
-    const float mean1 = more && mean_in ? __ldg(mean_in + row + step) : 0.f,
-                rstd1 = more ? __ldg(rstd_in + row + step) : 0.f;
+    const float mean1 = more && mean_in ? load_in_order(mean_in + row + step) : 0.f,
+                rstd1 = more ? load_in_order(rstd_in + row + step) : 0.f;
     // (a row or column that is not there is zero, and so is its dy: it adds nothing)
     const pair r = pack2(rstd, rstd), m = pack2(-mean, -mean);
     acc[0] = acc[1] = 0;
@@ -510,7 +519,7 @@ int forward_t(const T* x, const P* gamma, const P* beta, T* y, float* mean, floa
   const bool vec = s.d % VW == 0 && (s.x_stride * (int64_t)sizeof(T)) % 16 == 0 && aligned16(x) &&
                    aligned16(y) && aligned16(gamma) && aligned16(beta);
   int nv = s.d / VW;
-  if (vec) s.tpr = threads_per_row(nv, nv <= 64 ? 2 : nv <= 96 ? 3 : 4);
+  if (vec) s.tpr = threads_per_row(nv, VW == 4 ? 4 : nv <= 64 ? 2 : nv <= 96 ? 3 : 4);
   if (vec && s.tpr != 0) {
     const int vpt = ceil_div(nv, s.tpr);
     return vpt <= 1   ? forward_vpt<T, P, VW, 1>(x, gamma, beta, y, mean, rstd, s, sms, st)
@@ -557,7 +566,8 @@ int backward_t(const T* dy, const T* x, const P* gamma, const float* mean, const
                    (s.dy_stride * (int64_t)sizeof(T)) % 16 == 0 && aligned16(x) && aligned16(dy) &&
                    aligned16(dx) && aligned16(gamma);
   int nv = s.d / VW;
-  if (vec) s.tpr = threads_per_row(nv, nv <= 64 ? 2 : nv <= 96 ? 3 : nv <= 1024 ? 2 : 4);
+  // (16 elements a thread, 24 where a warp then has a bf16 row of 768: column sums and a row in 128 registers)
+  if (vec) s.tpr = threads_per_row(nv, VW == 4 ? 4 : nv <= 64 ? 2 : nv <= 96 ? 3 : nv <= 1024 ? 2 : 4);
   if (vec && s.tpr != 0) {
     const int vpt = ceil_div(nv, s.tpr);
     return vpt <= 1   ? backward_vpt<T, P, VW, 1>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)

@@ -636,7 +636,7 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // fp32 768 x 128 (786 KB) 256 tokens x 4 74 / 128, 400 tokens 111 / 119.
 bool takes_few(int64_t P, int d, int E, int H, int k, bool glu, int dtype, bool tiles) {
   const int64_t expert = (int64_t)(glu ? 3 : 2) * d * H * (dtype == D2D_F32 ? 4 : 2);
-  const int64_t most = tiles ? std::max<int64_t>(100 << 20, expert * E * 9 / 4) : 1200LL << 20;
+  const int64_t most = tiles ? std::max<int64_t>(100 << 20, expert * E * 9 / 4) : 1100LL << 20;
   return P <= 2048 && P * expert <= most && (size_t)k * H * sizeof(float) <= 64 * 1024;
 }
 
