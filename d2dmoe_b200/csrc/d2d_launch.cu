@@ -6,7 +6,7 @@
 namespace d2d {
 namespace {
 
-constexpr int MAX_DEVICES = 64, MAX_KERNELS = 64;
+constexpr int MAX_DEVICES = 64, MAX_KERNELS = 256;
 struct OptIn {
   const void* kernel;
   size_t smem;

@@ -740,14 +740,13 @@ int route_gradient(const at::Tensor& gt, const at::Tensor& lt, const at::Tensor&
 }
 
 // ---- the same under autograd ----------------------------------------------------------
-// First derivatives only: where the gradients' own graph is asked for, differentiating it says so.
+// First derivatives only: where the gradients' own graph is asked for, differentiating it says so, whatever the incoming
+// gradient is made of (the second derivative in the operator's own input would be left out without a word).
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-variable_list once(variable_list grads, const variable_list& incoming, const char* what) {
-  bool twice = at::GradMode::is_enabled(), any = false;
-  for (const at::Tensor& g : incoming) any |= g.defined() && g.requires_grad();
-  if (!twice || !any) return grads;
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
   for (at::Tensor& g : grads)
     if (g.defined()) g = g.detach().set_requires_grad(true);
   auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has first derivatives only",
@@ -777,7 +776,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const int rc = norm_backward(g[0], s[0], s[1].defined() ? &s[1] : nullptr, s[2].defined() ? &s[2] : nullptr, s[3], h,
                                  want, &out[0], &out[1], &out[2]);
     TORCH_CHECK(rc == D2D_OK, "d2d_layer_norm_backward: ", d2d_strerror(rc));
-    return once(std::move(out), g, "layer_norm");
+    return once(std::move(out), "layer_norm");
   }
 };
 
@@ -805,7 +804,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
     h.scale = ctx->saved_data["scale"].toDouble();
     const int rc = route_gradient(g[0], s[0], s[1], s[2], h, &out[0]);
     TORCH_CHECK(rc == D2D_OK, "d2d_route_backward: ", d2d_strerror(rc));
-    return once(std::move(out), g, "route_tokens");
+    return once(std::move(out), "route_tokens");
   }
 };
 
@@ -954,6 +953,10 @@ PyObject* run_weighted_experts(const ExpertWeights& m, const at::Tensor& xt, con
   if (bias) {
     of_type(*bias, xt.scalar_type(), "last_bias");
     TORCH_CHECK_VALUE(bias->numel() == m.d && bias->is_contiguous(), "last_bias must have ", m.d, " values");
+  }
+  if (status) {
+    of_type(*status, at::kInt, "status");
+    TORCH_CHECK_VALUE(status->numel() > 0, "status must have one value");
   }
   if (k < 1 || k > m.E) return PyLong_FromLong(D2D_ERR_BAD_ARG);
   On on(xt);

@@ -157,10 +157,18 @@ class _PackedCache:
         return self._buf
 
 
+def _not_in_a_capture():
+    """What a module keeps is not made in a capture: it would be there only once the graph has run."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("forward_weighted lays out its weights and its status word in the first call, and the weights "
+                           "again after they changed: make that call before the capture")
+
+
 class _StatusWords(dict):
     """Device status words of a module's weighted calls, one per device; copies start without any."""
 
     def __missing__(self, device):
+        _not_in_a_capture()
         w = self[device] = torch.zeros(1, dtype=torch.int32, device=device)
         return w
 
@@ -260,7 +268,8 @@ class B200KernelExperts(ExpertsLayer):
     def forward_weighted(self, x, experts, weights, last_bias=None, add_residual=False):
         """``last_bias (+ x) + sum_j weights[.., j] * expert_{experts[.., j]}(x)`` for x [.., d] and what
         ``route_tokens`` returns: experts [.., k] int32 (-1: no such slot), weights [.., k] fp32.  A token's sum is held in
-        fp32, in the order of its slots, and rounded once; the result has no gradient.  (Upstream multiplies every
+        fp32, in the order of its slots, and rounded once; the result has no gradient.  The first call, and the first after the weights changed, cannot be captured
+        in a graph.  (Upstream multiplies every
         expert's output by its routing entry, architectures/moe/moe_layers.py:91-101.)"""
         self._check_mode()
         if self._capture is not None:
@@ -281,15 +290,27 @@ class B200KernelExperts(ExpertsLayer):
                     raise D2DError(r, "d2d_experts_weighted")
                 if r is not None:
                     return r
+            self._image_before_capture()
             with torch.no_grad():
                 plan.handle = self._make_weighted_plan()
             if plan.handle is None:
                 break
+        if x.is_cuda:
+            self._image_before_capture()
         with torch.no_grad():
             p = self.kernel_params()
             return ops.experts_weighted(x, experts, weights, p["w1"], p["b1"], p["w2"], p["act"], w_up=p["w_up"],
                                         packed=self.packed(), last_bias=last_bias, add_residual=add_residual,
                                         status=status)
+
+    def _image_before_capture(self):
+        """Lay the weights out where they are not yet, unless the stream captures."""
+        if torch.cuda.is_current_stream_capturing():
+            image = self._packed._buf
+            with torch.no_grad():
+                if self.packed() is not image:
+                    self.invalidate_packed()
+                    _not_in_a_capture()
 
     def _make_weighted_plan(self):
         """Plan of ``forward_weighted`` for the parameters as they are now, or None where something but the plain

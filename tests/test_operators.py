@@ -1098,3 +1098,58 @@ def test_refusals_of_tensors():
             call()
             pytest.fail(f"call {n} was not refused")
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused_for_plain_incoming_gradients():
+    """y's gradient does not require one itself: the second derivative in x is there all the same."""
+    import d2dmoe_b200 as D
+    x, w, b, dy = norm_inputs(20, 96, "fp32", "same", "layer", 0)
+    leaf = x.detach().clone().requires_grad_()
+    for y in (D.layer_norm(leaf, w, b), D.route_tokens(leaf, 3)[0]):
+        g, = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            (g.square().sum() + y.sum()).backward()
+
+
+@pytest.mark.gpu
+def test_weighted_status_word_is_checked():
+    import d2dmoe_b200 as D
+    g = gen(5)
+    x, e, w = randn(g, 3, 64), torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, 1, device="cuda")
+    w1, w2 = randn(g, 2, 64, 32), randn(g, 2, 32, 64)
+    for status, error in ((torch.zeros(1, dtype=torch.int64, device="cuda"), TypeError),
+                          (torch.zeros(0, dtype=torch.int32, device="cuda"), ValueError)):
+        with pytest.raises(error, match="status"):
+            D.ops.experts_weighted(x, e, w, w1, None, w2, "relu", status=status)
+
+
+@pytest.mark.gpu
+def test_weighted_layouts_are_not_made_in_a_capture():
+    """The first call, and the first after the weights changed, lay out what later calls read: refused in a capture,
+    and right afterwards."""
+    import copy
+    ex = weighted_layer().experts
+    g = gen(6)
+    x, w = randn(g, 700, 256).bfloat16(), torch.rand(700, 4, device="cuda")
+    e = torch.randint(0, 24, (700, 4), device="cuda", dtype=torch.int32)
+
+    def refused():
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                ex.forward_weighted(x, e, w)
+
+    refused()
+    before = ex.forward_weighted(x, e, w)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = ex.forward_weighted(x, e, w)
+    gr.replay()
+    assert torch.equal(out, before)
+    with torch.no_grad():
+        ex.w2.mul_(2.0)
+    refused()
+    with torch.no_grad():
+        fresh = copy.deepcopy(ex).forward_weighted(x, e, w)
+    assert torch.equal(ex.forward_weighted(x, e, w), fresh) and not torch.equal(fresh, before)
+    ex.check_status()
