@@ -8,8 +8,9 @@
 //           run over the lists and store row p of a table [N k, d], and a last pass sums each token's k rows, which
 //           lie together.  That table is what bounds this form: it is written and read once (50432 tokens x 4 x 768:
 //           310 MB each way next to 155 MB of x and out).  The tensor-core kernel's rows are 16 bits an
-//           element, in a format of its own (encode8) that is off by 2^-14 of the largest of eight where bf16 would be by 2^-9; the
-//           general-shape kernel's are fp32.
+//           element, in a format of its own (encode8) that is off by 2^-14 of the largest of eight where bf16 would be by 2^-8 of each
+//           (error of a gated call against 64 bits 2.4e-3 instead of 2.8e-3 of the 2-norm, 1.7e-3 of it the result's own
+//           rounding); the general-shape kernel's are fp32.  50432 x 768, 4 of 24 experts: sort 11, experts 112, sum 78 us.
 //   few     Calls of few pairs are bound by latency and by the weights' bytes: two kernels without lists, all
 //           sums in 32 bits.  Blocks share out a pair's hidden columns in the first, a token's columns in the second;
 //           where those are fewer than the SMs take, clusters split the depth, or the slots, and meet in distributed
