@@ -287,6 +287,10 @@ int launch_router_fp32(const void* x, const void* wa, const void* wb, float mult
 int launch_experts_fp32(const void* x, const int32_t* token_idx, const int32_t* offsets,
                         const void* w1, const void* b1, const void* w2, void* out, int64_t N, int d,
                         int E, int H, int act, int* dev_status, cudaStream_t s, int kept);
+bool experts_fp32_pairs_supported(int d, int E, int H);
+int launch_experts_fp32_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,
+                              const void* b1, const void* w2, void* out, int64_t N, int d, int E, int H, int k,
+                              int act, int* dev_status, cudaStream_t s);
 bool experts_simt_fits(int H, bool glu);      // the general-shape kernel's shared memory
 // Lists of pairs p = token k + slot: out row p [d] fp32 = the expert's output for the token (see d2d_weighted.cu)
 int launch_experts_simt_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,

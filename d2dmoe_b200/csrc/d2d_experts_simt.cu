@@ -434,6 +434,10 @@ int launch_experts_simt_pairs(const void* x, const int32_t* pairs, const int32_t
                               const void* b1, const void* w_up, const void* w2, void* out, int64_t N, int d,
                               int E, int H, int k, int act, int dtype, int* dev_status, cudaStream_t s) {
   if (E > MAX_E) return D2D_ERR_UNSUPPORTED;
+  if (dtype == D2D_F32 && !w_up) {
+    const int rc = launch_experts_fp32_pairs(x, pairs, offsets, w1, b1, w2, out, N, d, E, H, k, act, dev_status, s);
+    if (rc != D2D_ERR_UNSUPPORTED) return rc;
+  }
   const auto launch = dtype == D2D_F32 ? (w_up ? launch_tm<float, true, 32, true> : launch_tm<float, false, 32, true>)
                                        : (w_up ? launch_tm<bf16, true, 32, true> : launch_tm<bf16, false, 32, true>);
   return launch(x, pairs, offsets, w1, b1, w_up, w2, out, N, d, E, H, act, dev_status, s, NormCapture(), k);

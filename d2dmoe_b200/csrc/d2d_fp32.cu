@@ -14,7 +14,7 @@
 //     two vectors, else 4, whatever is the same across the rest of the warp: hence the lanes' order.
 //   router   a cluster of four CTAs has 16 tokens; each takes every fourth slice of 32 hidden
 //            columns and the scores' share of it; the shares meet through distributed shared memory
-//   experts  an item is (expert, 16 or 32 rows of its list, 32 hidden columns); it adds its share of the
+//   experts  an item is (expert, 16 or 32 rows of its list, 32 hidden columns; in the weighted form all); it adds its share of the
 //            second product to the output rows.  In fp32 nothing is rounded between the
 //            slices, so no exchange is needed; the price is one add of the output rows per slice.
 // Measured (24 experts x 768 x 128, router 128, graph replays, stages that a CTA shares -> this): 50 tokens
@@ -40,6 +40,8 @@ constexpr int W2_ROWS = 8;         // second product: rows of W2 in a stage, 64 
 constexpr int CLUSTER = 4;
 constexpr int MAX_E = 256;
 constexpr int CP = TH + 4;         // row pitch of Wb's columns
+constexpr int PAIR_CTAS = 4;       // of an SM in the weighted form, with 128 hidden columns beside the stages
+constexpr int PAIR_MAX_H = 512;    // of it (32 KB of hidden values; the stages are 45)
 
 // MR: rows of a lane in either product, a quarter of an item's
 template <int MR>
@@ -121,10 +123,11 @@ struct Ring {
 };
 
 // Sums of the TR x 32 product, thread t: row t / (32 / MR), columns MR (t % (32 / MR)) .. + MR - 1.  issue(stage, s)
-// copies this warp's part of chunk s to that address (s >= chunks: what the caller wants next).  BT: the B tile is
-// [column][k] (b_col) instead of [k][column].
+// copies this warp's part of chunk s to that address (s >= chunks: what the caller wants next; primed: so did the
+// product before, for this one's first chunks).  BT: the B tile is [column][k] (b_col) instead of [k][column].
 template <int MR, bool BT, typename Issue>
-__device__ __forceinline__ void product(Ring<MR>& r, float* part, int chunks, Issue issue, float* sum) {
+__device__ __forceinline__ void product(Ring<MR>& r, float* part, int chunks, Issue issue, float* sum,
+                                        bool primed = false) {
   using T = Tiling<MR>;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int kh = lane >> 4, rg = (lane >> 1 & 1) | (lane >> 2 & 2), cg = (lane & 1) | (lane >> 1 & 2);
@@ -134,11 +137,13 @@ __device__ __forceinline__ void product(Ring<MR>& r, float* part, int chunks, Is
   for (int i = 0; i < MR; ++i)
 #pragma unroll
     for (int j = 0; j < (BT ? 8 : 4); ++j) sums[i][j] = 0;
+  if (!primed) {
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s) {
-    issue(r.fill, s);
-    r.fill = r.after(r.fill);
-    cp_commit();
+    for (int s = 0; s < ST - 1; ++s) {
+      issue(r.fill, s);
+      r.fill = r.after(r.fill);
+      cp_commit();
+    }
   }
   // (vectors 2 kk + kh: the swizzle leaves the low bit alone)
   const uint32_t a0 = 4 * at_k(rg, kh), a1 = 4 * at_k(rg, 2 + kh);
@@ -400,22 +405,30 @@ router_fp32_kernel(const float* __restrict__ x, const float* __restrict__ wa,
 // ---------------------------------------------------------------------------
 // experts
 // ---------------------------------------------------------------------------
-template <int MR>
-__global__ void __launch_bounds__(NT, Tiling<MR>::CTAS)
+// FORM of the lists: of tokens, whose items add to rows of out; or of pairs p = token * slots + slot (the weighted form), whose
+// items have all of H and store row p of out: the same bits every time.  SPLIT: an item is a cluster's, each CTA computes
+// some slices of the hidden values, hands them to all through distributed shared memory, and multiplies all of them by
+// its share of W2's columns, 64 a warp.
+enum Form { TOKENS, WHOLE, SPLIT };
+template <int MR, int FORM>
+__global__ void __launch_bounds__(NT, FORM ? PAIR_CTAS : Tiling<MR>::CTAS)
 experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ token_idx,
                     const int32_t* __restrict__ offsets, const float* __restrict__ w1,
                     const float* __restrict__ b1, const float* __restrict__ w2,
                     float* __restrict__ out, int64_t N, int d, int E, int H, int act,
-                    int* dev_status) {
+                    int* dev_status, int slots) {
   using T = Tiling<MR>;
   constexpr int TR = T::TR;
+  constexpr bool PAIRS = FORM != TOKENS;
   extern __shared__ __align__(16) float sm[];
-  float* hs = sm + 4 * ST * T::STAGE;         // sums, then [TR][TH] hidden slice in the first warp's
-  int* off = reinterpret_cast<int*>(sm + T::FLOATS);      // [E + 1]
+  float* part = sm + 4 * ST * T::STAGE;       // sums, then [TR][TH] hidden slice in the first warp's
+  float* hs = PAIRS ? sm + T::FLOATS : part;  // (PAIRS: [slice][TR][TH])
+  int* off = reinterpret_cast<int*>(sm + T::FLOATS + (PAIRS ? (H + TH - 1) / TH * TR * TH : 0));      // [E + 1]
   int* tstart = off + E + 1;                              // [E + 1] first tile of each expert
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
+  if (PAIRS) fresh(x, token_idx, offsets, w1, b1, w2);
   for (int e = tid; e <= E; e += NT) off[e] = offsets[e];
   __syncthreads();
   if (w == 0) {                        // lane has experts 8 lane .. + 7
@@ -445,11 +458,18 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
     if (lane == 31) tstart[E] = incl;
   }
   __syncthreads();
-  const int slices = (H + TH - 1) / TH, chunks = (d + KC - 1) / KC, total = tstart[E] * slices;
+  const int slices = PAIRS ? 1 : (H + TH - 1) / TH, chunks = (d + KC - 1) / KC, total = tstart[E] * slices;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = FORM == SPLIT ? (int)cluster.num_blocks() : 1, rank = FORM == SPLIT ? (int)cluster.block_rank() : 0;
+  const int all = (H + TH - 1) / TH, blocks = (d + 63) / 64;
+  const int ha = all * rank / ctas * TH, hb = min(all * (rank + 1) / ctas * TH, H);       // (PAIRS) this CTA's slices
+  const int ca = blocks * rank / ctas, cb = blocks * (rank + 1) / ctas;                   // and columns
+  if constexpr (FORM == SPLIT) cluster.sync();   // (all have started: their memory may be written to)
+  bool read = false;                   // (SPLIT) the hidden values of an item before this one may still be read
   const int lr = lane >> 2, kl = w * KW + 4 * (lane & 3), dst = at_k(lr, lane & 3);
 #pragma unroll 1
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const int tile = item / slices, h0 = (item - tile * slices) * TH;
+  for (int item = blockIdx.x / ctas; item < total; item += gridDim.x / ctas) {
+    const int tile = item / slices, h0 = PAIRS ? ha : (item - tile * slices) * TH;
     int lo = 0, hi = E;                // last e with tstart[e] <= tile
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -458,27 +478,31 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
     const int e = lo, r0 = off[e] + (tile - tstart[e]) * TR;
     const int nrows = min(TR, off[e + 1] - r0);
     int tok = lane < nrows ? token_idx[r0 + lane] : -1;   // every warp has the item's rows
-    if (lane < nrows && (tok < 0 || tok >= N)) {
+    if (lane < nrows && (tok < 0 || tok >= (PAIRS ? N * slots : N))) {
       if (w == 0) report(dev_status, D2D_ERR_INDEX_RANGE);
       tok = -1;
     }
+    const int x_row = PAIRS ? max(tok, 0) / slots : tok;
     // the rows of x and the columns of the weights this lane copies, one chunk after another (in the place of
     // what is not there: the first ones, whose sums nobody uses)
     const float* xr[TR / 8];
 #pragma unroll
     for (int u = 0; u < TR / 8; ++u)
-      xr[u] = x + (int64_t)max(__shfl_sync(0xffffffffu, tok, lr + 8 * u), 0) * d + kl;
-    const int kn = min(TH, H - h0), pieces = (kn + W2_ROWS - 1) / W2_ROWS;
+      xr[u] = x + (int64_t)max(__shfl_sync(0xffffffffu, x_row, lr + 8 * u), 0) * d + kl;
+    const int kn = PAIRS ? H : min(TH, H - h0), pieces = (kn + W2_ROWS - 1) / W2_ROWS;
     const float* w1r = w1 + ((int64_t)e * d + w * KW + (lane >> 3)) * H + h0 +
-                       (4 * (lane & 7) < kn ? 4 * (lane & 7) : 0);
-    const float* const w2s = w2 + ((int64_t)e * H + h0 + (lane >> 4)) * d;
-    const float* w2r = w2s + min(64 * w + 4 * (lane & 15), d - 4);
+                       (4 * (lane & 7) < (PAIRS ? H - h0 : kn) ? 4 * (lane & 7) : 0);
+    const float* const w2s = w2 + ((int64_t)e * H + (PAIRS ? 0 : h0) + (lane >> 4)) * d;
+    const int end = PAIRS ? 64 * (cb - w) : d;       // of p_next
+    int p_next = PAIRS ? 64 * ca : 0, k_next = 0;    // columns and rows of W2 that are copied next
+    const float* w2r = w2s + min(p_next + 64 * w + 4 * (lane & 15), d - 4);
     const uint32_t dst1 = 4 * (T::A_FLOATS + (lane >> 3) * TH + 4 * (lane & 7)),
                    dst1x = 4 * (T::A_FLOATS + (lane >> 3) * TH + 4 * ((lane & 7) ^ 4)),
                    dst2 = 4 * ((lane >> 4) * 64 + 4 * (lane & 15));
-    int p_next = 0, k_next = 0;        // columns and rows of W2 that are copied next
+    int c_next = 0, h_next = h0;       // (PAIRS) chunk and hidden slice of W1
     auto issue = [&](uint32_t stage, int s) {
-      if (s < chunks) {
+      if (PAIRS) s = c_next;
+      if (PAIRS ? h_next < hb : s < chunks) {
         const float* row = w1r;
         const int64_t four = 4 * (int64_t)H;
         if (s * KC + KC <= d) {
@@ -500,7 +524,15 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
 #pragma unroll
         for (int u = 0; u < TR / 8; ++u) xr[u] += KC;
         w1r += (int64_t)KC * H;
-      } else if (p_next < d) {
+        if (PAIRS && ++c_next == chunks) {           // x again, for the next slice
+          c_next = 0;
+          h_next += TH;
+#pragma unroll
+          for (int u = 0; u < TR / 8; ++u) xr[u] -= (int64_t)chunks * KC;
+          w1r = w1 + ((int64_t)e * d + w * KW + (lane >> 3)) * H + h_next +
+                (4 * (lane & 7) < H - h_next ? 4 * (lane & 7) : 0);
+        }
+      } else if (p_next < end) {
         const float* row = w2r;
         const int64_t two = 2 * (int64_t)d;
         if (k_next + W2_ROWS <= kn) {
@@ -522,29 +554,45 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
         }
       }
     };
-    float h[MR];
     Ring<MR> ring(sm + w * ST * T::STAGE);
-    product<MR, false>(ring, hs, chunks, issue, h);
-    const int row = tid / (32 / MR), v0 = (MR / 4) * (tid % (32 / MR));
+    auto hidden = [&](int hc, bool primed) {         // columns hc .. hc + 31
+      float h[MR];
+      product<MR, false>(ring, part, chunks, issue, h, primed);
+      const int row = tid / (32 / MR), v0 = (MR / 4) * (tid % (32 / MR));
 #pragma unroll
-    for (int u = 0; u < MR / 4; ++u) {
+      for (int u = 0; u < MR / 4; ++u) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = h0 + 4 * (v0 + u) + q;
-        float v = 0.f;
-        if (c < H)
-          v = activate(b1 ? h[4 * u + q] + __ldg(b1 + (int64_t)e * H + c) : h[4 * u + q], act);
-        h[4 * u + q] = v;
+        for (int q = 0; q < 4; ++q) {
+          const int c = hc + 4 * (v0 + u) + q;
+          float v = 0.f;
+          if (c < H)
+            v = activate(b1 ? h[4 * u + q] + __ldg(b1 + (int64_t)e * H + c) : h[4 * u + q], act);
+          h[4 * u + q] = v;
+        }
+        float* const at = hs + (PAIRS ? hc * TR : 0) + at_h(row, v0 + u);
+        const float4 v4 = make_float4(h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+        if constexpr (FORM == SPLIT) {
+          if (u == 0 && read) cluster.barrier_wait();
+          read = false;
+          for (int c = 0; c < ctas; ++c) *reinterpret_cast<float4*>(cluster.map_shared_rank(at, c)) = v4;
+        } else {
+          *reinterpret_cast<float4*>(at) = v4;
+        }
       }
-      *reinterpret_cast<float4*>(hs + at_h(row, v0 + u)) =
-          make_float4(h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+      __syncthreads();
+    };
+    if constexpr (PAIRS) {
+#pragma unroll 1
+      for (int hc = h0; hc < hb; hc += TH) hidden(hc, hc > h0);
+      if constexpr (FORM == SPLIT) cluster.sync();
+    } else {
+      hidden(h0, false);
     }
-    __syncthreads();
     // second product: TR rows x 256 columns per pass, K = 32; a warp has 64 columns, a lane MR x 8
     const uint32_t hs0 = smem_addr(hs);
     const int rg = (lane >> 1 & 1) | (lane >> 3 & 2), cgp = (lane & 1) | (lane >> 1 & 6);
 #pragma unroll 1
-    for (int p0 = 0; p0 < d; p0 += 256) {
+    for (int p0 = PAIRS ? 64 * ca : 0; p0 < end; p0 += 256) {
       pair sums[MR][4];
 #pragma unroll
       for (int i = 0; i < MR; ++i)
@@ -563,7 +611,8 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
           float a[MR][4];
 #pragma unroll
           for (int i = 0; i < MR; ++i)
-            ld_vec(hs0 + 4 * at_h(rg + 4 * i, kp * (W2_ROWS / 4) + kk), a[i]);
+            ld_vec(hs0 + (PAIRS ? 4 * TR * TH * (kp >> 2) : 0) +
+                       4 * at_h(rg + 4 * i, (PAIRS ? kp & 3 : kp) * (W2_ROWS / 4) + kk), a[i]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             pair b[4];
@@ -587,29 +636,45 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
         float* o = out + (int64_t)t * d + c0;
         const float2 f0 = halves(sums[i][0]), f1 = halves(sums[i][1]);
         const float2 f2 = halves(sums[i][2]), f3 = halves(sums[i][3]);
+        if (PAIRS) {
+          if (c0 < d) *reinterpret_cast<float4*>(o) = make_float4(f0.x, f0.y, f1.x, f1.y);
+          if (c0 + 32 < d) *reinterpret_cast<float4*>(o + 32) = make_float4(f2.x, f2.y, f3.x, f3.y);
+          continue;
+        }
         if (c0 < d) red_add_v4(o, f0.x, f0.y, f1.x, f1.y);
         if (c0 + 32 < d) red_add_v4(o + 32, f2.x, f2.y, f3.x, f3.y);
       }
     }
-    __syncthreads();                   // the hidden slice has been read
+    if constexpr (FORM == SPLIT) {     // the hidden values have been read
+      __syncwarp();
+      cluster.barrier_arrive();
+      read = true;
+    } else {
+      __syncthreads();                 // the hidden slice has been read
+    }
   }
+  if (FORM == SPLIT && read) cluster.barrier_wait();         // (none may be gone while another writes to its memory)
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int MR>
+template <int MR, int FORM>
 int launch_experts(const float* x, const int32_t* token_idx, const int32_t* offsets, const float* w1,
                    const float* b1, const float* w2, float* out, int64_t N, int d, int E, int H,
-                   int act, int* dev_status, int sms, cudaStream_t s) {
+                   int act, int* dev_status, int sms, cudaStream_t s, int slots = 1, int cluster = 1) {
   using T = Tiling<MR>;
-  const size_t smem = sizeof(float) * (size_t)T::FLOATS + 2 * sizeof(int) * (size_t)(E + 1);
-  const int rc = device_launch_facts((const void*)experts_fp32_kernel<MR>, smem, nullptr);
+  const int slices = ceil_div(H, TH);
+  const size_t smem = sizeof(float) * ((size_t)T::FLOATS + (FORM ? (size_t)slices * T::PART : 0)) +
+                      2 * sizeof(int) * (size_t)(E + 1);
+  const auto kernel = experts_fp32_kernel<MR, FORM>;
+  const int rc = device_launch_facts((const void*)kernel, smem, nullptr);
   if (rc != D2D_OK) return rc;
   // at most one item per TR rows of an expert and slice, plus a partial one
-  const int64_t most = (ceil_div64(N * (int64_t)E, T::TR) + E) * ceil_div(H, TH);
-  const int64_t ctas = (int64_t)T::CTAS * sms, grid = most < ctas ? most : ctas;
-  return launch_pdl(experts_fp32_kernel<MR>, dim3((unsigned)grid), dim3(NT), smem, s, x, token_idx,
-                    offsets, w1, b1, w2, out, N, d, E, H, act, dev_status);
+  const int64_t most =
+      FORM ? (ceil_div64(N * slots, T::TR) + E) * cluster : (ceil_div64(N * (int64_t)E, T::TR) + E) * slices;
+  const int64_t ctas = (int64_t)(FORM ? PAIR_CTAS : T::CTAS) * sms / cluster * cluster, grid = most < ctas ? most : ctas;
+  return launch_pdl_cluster(FORM == SPLIT ? cluster : 0, kernel, dim3((unsigned)grid), dim3(NT), smem, s, x, token_idx,
+                            offsets, w1, b1, w2, out, N, d, E, H, act, dev_status, slots);
 }
 
 }  // namespace
@@ -661,9 +726,35 @@ int launch_experts_fp32(const void* x, const int32_t* token_idx, const int32_t* 
   const bool rows32 = kept ? pairs >= 400 * (int64_t)E ||
                                  11 * rounds(32, Tiling<8>::CTAS) <= 10 * rounds(16, Tiling<4>::CTAS)
                            : pairs >= 288 * (int64_t)E;
-  auto launch = rows32 ? launch_experts<8> : launch_experts<4>;
+  const auto launch = rows32 ? launch_experts<8, TOKENS> : launch_experts<4, TOKENS>;
   return launch((const float*)x, token_idx, offsets, (const float*)w1, (const float*)b1,
-                (const float*)w2, (float*)out, N, d, E, H, act, dev_status, sms, s);
+                (const float*)w2, (float*)out, N, d, E, H, act, dev_status, sms, s, 1, 1);
+}
+
+bool experts_fp32_pairs_supported(int d, int E, int H) {
+  return d % 4 == 0 && H % 4 == 0 && E <= MAX_E && H <= PAIR_MAX_H;
+}
+
+// The weighted form: lists of pairs, fp32 rows of out (a row per pair) stored.  Items of 16 rows (of 32, us, 16 / 32:
+// 1576 tokens x 4 of 24 experts x 128 106 / 102, 2400 130 / 142, 3152 152 / 143, 4700 230 / 237), each for a CTA, or for
+// clusters of two or four where these all run at a time: a CTA alone takes 55 us for an item whose FMAs are 13.
+// d = 768, 24 x 128, us, alone / two / four: 400 tokens 71 / 60 / 44, 788 84 / 68 / 67, 1200 105 / 81 / 89, 1576 105 / 118 / 109,
+// 2400 130 / 138 / 186; d = 1024, 16 x 512, top-2: 788 270 / 150 / 153, 3152 424 / 422 / 478.  (With the sort and the sum,
+// 17 us of each.  The general-shape kernel: 139 for 1576 tokens.)
+int launch_experts_fp32_pairs(const void* x, const int32_t* pairs, const int32_t* offsets, const void* w1,
+                              const void* b1, const void* w2, void* out, int64_t N, int d, int E, int H, int k,
+                              int act, int* dev_status, cudaStream_t s) {
+  if (!experts_fp32_pairs_supported(d, E, H) || !al16(x) || !al16(w1) || !al16(w2) || !al16(out))
+    return D2D_ERR_UNSUPPORTED;
+  int sms = 0;
+  const int rc = device_launch_facts(nullptr, 0, &sms);
+  if (rc != D2D_OK) return rc;
+  const int64_t items = ceil_div64(N * k, Tiling<4>::TR) + E / 2;           // half of one more for each list
+  int cluster = 4;
+  while (cluster > 1 && (cluster > ceil_div(H, TH) || 16 * items * cluster > 17 * (int64_t)PAIR_CTAS * sms)) cluster /= 2;
+  const auto launch = cluster > 1 ? launch_experts<4, SPLIT> : launch_experts<4, WHOLE>;
+  return launch((const float*)x, pairs, offsets, (const float*)w1, (const float*)b1, (const float*)w2, (float*)out, N, d,
+                E, H, act, dev_status, sms, s, k, cluster);
 }
 
 }  // namespace d2d

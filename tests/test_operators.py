@@ -1153,3 +1153,37 @@ def test_weighted_layouts_are_not_made_in_a_capture():
         fresh = copy.deepcopy(ex).forward_weighted(x, e, w)
     assert torch.equal(ex.forward_weighted(x, e, w), fresh) and not torch.equal(fresh, before)
     ex.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # N, d, E, H, k, biases: items of one CTA, of two and of four; one slice of hidden columns and sixteen, the last one
+    # of four columns; one chunk of d and several; fewer 64-column blocks than CTAs; more items than run at a time
+    (550, 768, 24, 128, 4, True), (1200, 768, 24, 128, 4, True), (3200, 768, 24, 128, 4, False),
+    (2100, 68, 1, 100, 1, True), (2060, 64, 3, 160, 1, True), (1100, 4, 5, 36, 2, True), (2100, 132, 7, 512, 1, False),
+    (2100, 36, 3, 4, 1, True), (3400, 68, 200, 64, 1, True), (2100, 200, 9, 516, 1, True),
+    # the line between the two forms of few pairs and of lists
+    (108, 768, 24, 128, 4, True), (116, 768, 24, 128, 4, True)], ids=str)
+def test_weighted_experts_fp32_forms(case):
+    import d2dmoe_b200 as D
+    N, d, E, H, k, biases = case
+    x, e, w, w1, b1, w2, _, lb = experts_case(N, d, E, H, k, "fp32", False, biases)
+    if E == 200:         # 17 each: two items where one is expected and a half
+        e = (torch.arange(N, device="cuda") % E).int().view(N, 1)
+    e[3] = -1
+    if k > 1:
+        e[5] = e[5, 0]                                   # one expert several times
+        e[::7, 1] = -1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for act in ("relu", "gelu"):
+        want, tol = experts_reference(x, e, w, w1, b1, w2, act, None, lb, act == "relu")
+        args = dict(last_bias=lb, add_residual=act == "relu", status=status)
+        got = D.ops.experts_weighted(x, e, w, w1, b1, w2, act, **args)
+        within(got, want, tol, act)
+        for _ in range(3):
+            assert torch.equal(got, D.ops.experts_weighted(x, e, w, w1, b1, w2, act, **args))
+        # weights that start anywhere
+        off = torch.zeros(w1.numel() + 1, device="cuda")[1:].view(w1.shape)
+        off.copy_(w1)
+        within(D.ops.experts_weighted(x, e, w, off, b1, w2, act, **args), want, tol, "misaligned weights")
+    assert int(status.item()) == 0
