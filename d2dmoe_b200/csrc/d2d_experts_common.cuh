@@ -118,9 +118,9 @@ __device__ __forceinline__ void add_row(void* p, int t, uint4 v) {
       : "memory");
 }
 
-// Eight floats in 16 bytes: 15-bit integers in units of 2^(ex - 140) / (1 - 2^-14), where 2^(ex - 127) is the largest's power
+// Eight floats in 16 bytes: 15-bit integers in units of 2^(ex - 140) / (1 - 2^-15), where 2^(ex - 127) is the largest's power
 // of two: off by half a unit, 2^-14 of the largest of eight (bf16, as many bytes, would be by 2^-8 of each).  The
-// last factor keeps them below 2^14; they are held with 2^14 added.  The exponent lies in the upper bits of the
+// last factor keeps them below 2^14 - 1/2, so that none is rounded to 2^14; they are held with 2^14 added.  The exponent lies in the upper bits of the
 // eight halves.  Exponent 255, where one is not finite: the halves are the upper 15 bits of bf16.
 struct Eight {
   uint32_t f[8];           // bits of floats
@@ -145,7 +145,7 @@ __device__ __forceinline__ uint4 with_exponent(uint32_t a, uint32_t b, uint32_t 
 // ex: exponent8(v), below 255
 __device__ __forceinline__ uint4 encode8(const Eight& v, uint32_t ex) {
   ex = max(ex, 14u);
-  const float s = __uint_as_float(((266u - ex) << 23) + 0x7ffe00u);      // 2^(140 - ex) (1 - 2^-14): |f s| <= 2^14 - 1
+  const float s = __uint_as_float(((266u - ex) << 23) + 0x7ffe00u);      // 2^(139 - ex) (2 - 2^-14)
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {                              // 1.5 2^23 + 2^14: the integer is in the lower half
@@ -175,7 +175,7 @@ __device__ __forceinline__ uint32_t exponent_of(uint4 v) {
   return (y | y >> 15) & 255u;
 }
 // sum += wt * the eight (pairs of floats); ex: exponent_of(v); wt: with UNIT8 multiplied in
-constexpr float UNIT8 = 1.00006103888177f;                   // 1 / (1 - 2^-14)
+constexpr float UNIT8 = 1.00003051850948f;                   // 1 / (1 - 2^-15)
 __device__ __forceinline__ void add_decoded8(uint4 v, uint32_t ex, float wt, unsigned long long (&sum)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   const float s = wt * __uint_as_float((ex - 13u) << 23);    // 2^(ex - 140)
