@@ -318,14 +318,15 @@ struct Row {
     }
   }
   // Keys in the order of the logits: ordered logit, its `low` bits replaced by those of ~expert.  -inf (and what is not
-  // there) is below NO_KEY.
+  // there) is below NO_KEY.  Adding +0 makes one of both zeros, which are equal.
   __device__ __forceinline__ void keys(uint32_t* key, uint32_t low, int q) const {
     if constexpr (PACKED) {
 #pragma unroll
       for (int i = 0; i < WORDS; ++i) {
-        uint32_t sign;                                                       // of each half, all over it
-        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(sign) : "r"(w[i]));
-        const uint32_t o = w[i] ^ (sign | 0x80008000u);
+        uint32_t l, sign;                                                    // of each half, all over it
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(l) : "r"(w[i]), "r"(0u));
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(sign) : "r"(l));
+        const uint32_t o = l ^ (sign | 0x80008000u);
         const uint32_t e = ~(uint32_t)expert(2 * i, q);                      // (2 i + 1: one less)
         key[2 * i] = o << 16 | (e & low);
         key[2 * i + 1] = (o & 0xffff0000u) | ((e - 1u) & low);
@@ -333,7 +334,8 @@ struct Row {
     } else {
 #pragma unroll
       for (int i = 0; i < EL; ++i) {
-        const uint32_t e = (uint32_t)expert(i, q), o = w[i] ^ (0x80000000u | (uint32_t)((int32_t)w[i] >> 31));
+        const uint32_t e = (uint32_t)expert(i, q), l = __float_as_uint(__fadd_rn(__uint_as_float(w[i]), 0.f));
+        const uint32_t o = l ^ (0x80000000u | (uint32_t)((int32_t)l >> 31));
         key[i] = (o & ~low) | (~e & low);
       }
     }

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_operators import U, gen, half, randn, within
+from test_operators import DT, U, check_route, gen, half, randn, within
 
 
 # -- rows of pairs ------------------------------------------------------------------------------
@@ -41,3 +41,26 @@ def test_rows_of_pairs_keep_their_size(glu):
         size += float((y * y).sum())
     # 3072 errors of at most 2^-14 of about twice the value, either way: 2^-13 / sqrt(3 * 3072) = 1.3e-6 of the whole
     assert abs(along / size) <= 1e-5
+
+
+# -- zeros of both signs ------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("E,k", [(2, 1), (7, 3), (24, 1), (24, 8), (24, 4), (64, 16), (96, 12), (128, 8), (130, 8),
+                                 (256, 8), (1023, 16), (1024, 8), (40, 17)])
+def test_route_between_zeros_of_both_signs(E, k, dtype):
+    """-0 and +0 are equal: the lowest index is taken."""
+    g = gen(E + k)
+    N = 150
+    kind = torch.rand(N, E, generator=g, device="cuda")
+    size = randn(g, N, E).abs() + 0.1
+    zero = torch.where(torch.rand(N, E, generator=g, device="cuda") < 0.5, 0.0, -0.0)
+    size[:20] *= 2.0 ** -128                             # numbers below the normal ones beside the zeros
+    # fewer than k above the zeros, the others among them
+    logits = torch.where(kind < 0.4 * k / E, size, torch.where(kind < 0.9, zero, -size)).to(DT[dtype])
+    assert (torch.signbit(logits) & (logits == 0)).any()
+    for how in (dict(), dict(scores="sigmoid"), dict(renormalise=False)):
+        check_route(logits, k, randn(g, N, k), **how)
+    if E % 4 == 0 and k <= E // 2:
+        check_route(logits, k, groups=4, top_groups=2)
+        check_route(logits, k, groups=4, top_groups=3, scores="sigmoid", renormalise=False)
