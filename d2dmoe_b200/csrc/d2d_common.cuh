@@ -94,10 +94,16 @@ __device__ __forceinline__ void report(int* dev_status, int code) {
 }
 
 // ---- activations ----------------------------------------------------------
-// relu, exact-erf gelu, tanh, leaky relu (slope 0.01), tanh-form gelu.
+// the larger, NaN if either is (fmaxf would return the other)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// relu, exact-erf gelu, tanh, leaky relu (slope 0.01), tanh-form gelu; NaN stays NaN in all of them.
 __device__ __forceinline__ float activate(float h, int act) {
   switch (act) {
-    case D2D_RELU: return fmaxf(h, 0.0f);
+    case D2D_RELU: return max_nan(h, 0.0f);
     case D2D_GELU: return h * 0.5f * (1.0f + erff(h * 0.70710678118654752440f));
     case D2D_TANH: return tanhf(h);
     case D2D_LEAKY_RELU: return h >= 0.0f ? h : 0.01f * h;

@@ -70,7 +70,7 @@ __device__ __forceinline__ void ep1_pairs(const uint32_t* v, const uint32_t* u, 
         __floats2bfloat162_rn(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
     h = __hadd2_rn(h, *reinterpret_cast<const __nv_bfloat162*>(&bp[q]));
     if (ACT == D2D_RELU) {
-      h = __hmax2(h, __float2bfloat162_rn(0.f));
+      h = __hmax2_nan(h, __float2bfloat162_rn(0.f));
     } else {
       const float2 f = __bfloat1622float2(h);
       h = __floats2bfloat162_rn(activate(f.x, ACT), activate(f.y, ACT));

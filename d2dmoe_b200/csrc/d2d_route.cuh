@@ -70,12 +70,6 @@ __device__ __forceinline__ float reciprocal_fast(float v) {
 // e^(l - m): 2 ulp and |l - m| half ulps off
 __device__ __forceinline__ float softmax_term(float l, float m) { return exp2_fast((l - m) * LOG2E); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // -- what a choice gives: lane q of the L that have token t holds slots q, q + L, .. (e < 0: none) --------------
 // (the shuffles are for whole warps: a token that is not there, or made again, goes along with write = false)
 template <typename T, int L, int R>

@@ -1,9 +1,11 @@
 """Norm, routing and weighted experts on values and calls where a plain implementation is easily right: rows in their
 16-bit form, zeros of both signs, NaN through an activation, biases that cancel, rows wider than 2^16, tangents, streams."""
+import math
+
 import pytest
 import torch
 
-from test_operators import DT, U, check_route, gen, half, randn, within
+from test_operators import ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, within
 
 
 # -- rows of pairs ------------------------------------------------------------------------------
@@ -64,3 +66,48 @@ def test_route_between_zeros_of_both_signs(E, k, dtype):
     if E % 4 == 0 and k <= E // 2:
         check_route(logits, k, groups=4, top_groups=2)
         check_route(logits, k, groups=4, top_groups=3, scores="sigmoid", renormalise=False)
+
+
+# -- NaN and the activations ----------------------------------------------------------------------------
+# N x 3 pairs; packed; weights off a 16-byte boundary: few pairs, lists on the tensor cores, lists of the general kernel, fp32 lists
+FORMS = [("bf16", 5, True, False, False), ("bf16", 900, True, False, False), ("bf16", 900, False, False, False),
+         ("bf16", 5, True, True, False), ("bf16", 900, True, True, False), ("fp32", 5, False, False, False),
+         ("fp32", 900, False, False, False), ("fp32", 900, False, False, True), ("fp32", 900, False, True, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_a_nan_stays_one_through_every_activation(form, act):
+    import d2dmoe_b200 as D
+    dtype, N, pack, glu, off = form
+    x, e, w, w1, b1, w2, up, _ = experts_case(N, 128, 12, 32, 3, dtype, glu, not glu, seed=7)
+    x[2, 7] = math.nan
+    if off:
+        far = torch.zeros(w1.numel() + 1, dtype=w1.dtype, device="cuda")[1:].view(w1.shape)
+        w1 = far.copy_(w1)
+    packed = D.ops.prepack_experts(w1, b1, w2, up) if pack else None
+    assert (packed is not None) == pack
+    got = D.ops.experts_weighted(x, e, w, w1, b1, w2, act, w_up=up, packed=packed)
+    want, tol = experts_reference(x, e, w, w1, b1, w2, act, up)
+    assert torch.isnan(want[2]).all() and torch.isnan(got[2]).all()
+    keep = torch.arange(N, device="cuda") != 2
+    assert torch.isfinite(got[keep]).all()
+    within(got[keep], want[keep], tol[keep], "other rows")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [5, 150, 900])
+@pytest.mark.parametrize("dtype,d,H", [("bf16", 128, 32), ("bf16", 100, 20), ("fp32", 128, 32), ("fp32", 102, 33)])
+def test_a_nan_stays_one_through_the_unweighted_layer(dtype, d, H, N):
+    import d2dmoe_b200 as D
+    moe = D.MoeficationMoE("ffn", d, 12, True, H, torch.nn.ReLU).to(DT[dtype]).cuda().eval()
+    with torch.no_grad():
+        for p in moe.parameters():
+            p.copy_(randn(gen(p.numel()), *p.shape) / 8)
+    x = randn(gen(N), 1, N, d).to(DT[dtype])
+    x[0, 2, 7] = math.nan
+    out = moe(x)[0].detach()                             # every expert on every token
+    assert torch.isnan(out[0, 2]).all()
+    out[0, 2] = 0.0
+    assert torch.isfinite(out).all()
