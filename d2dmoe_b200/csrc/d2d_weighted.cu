@@ -233,7 +233,8 @@ __device__ __forceinline__ bool by_fours(const int32_t* e, const float* w, int k
   return k % 4 == 0 && ((reinterpret_cast<uintptr_t>(e) | reinterpret_cast<uintptr_t>(w)) & 15) == 0;
 }
 
-// y: [N k, d] fp32.  A thread has V columns of a token; a block takes a few tokens.  per_row: ceil(2^32 / (d / V))
+// y: [N k, d] fp32.  A thread has V columns of a token; a block takes a few tokens.  per_row: ceil(2^32 / (d / V)), for
+// quotients of numbers below 2 NT (where a token has more columns than that, it is the block's only one)
 template <typename T, int V>
 __global__ void __launch_bounds__(NT)
 combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ experts, const float* __restrict__ weights,
@@ -247,7 +248,7 @@ combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ experts,
   const int items = (int)min((int64_t)tokens, N - t0) * nv;
   const bool fours = by_fours(experts, weights, k);
   for (int i = threadIdx.x; i < items; i += NT) {
-    const int dt = nv == 1 ? i : (int)__umulhi((uint32_t)i, per_row), c = (i - dt * nv) * V;
+    const int dt = tokens == 1 ? 0 : nv == 1 ? i : (int)__umulhi((uint32_t)i, per_row), c = (i - dt * nv) * V;
     const int64_t t = t0 + dt;
     const float* row = y + t * k * d + c;
     float sum[V], f[V];

@@ -111,3 +111,23 @@ def test_a_nan_stays_one_through_the_unweighted_layer(dtype, d, H, N):
     assert torch.isnan(out[0, 2]).all()
     out[0, 2] = 0.0
     assert torch.isfinite(out).all()
+
+
+# -- rows wider than 2^16 -----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [("fp32", 70001), ("bf16", 100003)])
+def test_sum_of_rows_wider_than_a_quotients_range(dtype, d):
+    """Odd widths past 2^16 in lists (one thread a column): the last columns are their own token's."""
+    import d2dmoe_b200 as D
+    N, H = 2060, 4
+    x, e, w, w1, b1, w2, _, lb = experts_case(N, d, 3, H, 1, dtype, False, True)
+    x[:, 64:] = 0.0                                      # (sums of 64 terms)
+    w.uniform_(0.5, 2.0, generator=gen(8))
+    got = D.ops.experts_weighted(x, e, w, w1, b1, w2, "relu", last_bias=lb)
+    for t in (0, 1, 1000, N - 2, N - 1):
+        i = int(e[t, 0])
+        h = torch.relu(x[t, :64].double() @ w1[i, :64].double() + b1[i].double())
+        h_abs = x[t, :64].double().abs() @ w1[i, :64].double().abs() + b1[i].double().abs()
+        want = float(w[t, 0]) * (h @ w2[i].double()) + lb.double()
+        size = float(w[t, 0]) * (h_abs @ w2[i].double().abs()) + lb.double().abs()
+        within(got[t], want, half(DT[dtype]) * want.abs() + (2 * 64 + H + 16) * U * size, t)
