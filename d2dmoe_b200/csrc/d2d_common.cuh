@@ -50,7 +50,8 @@ __device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 // A pointer to what earlier kernels have written, behind the wait.  Loads that the compiler takes to be of constant
-// memory (__ldg, const __restrict__) do not heed the wait's clobber: without this it may move them above it.
+// memory (__ldg, const __restrict__) do not heed the wait's clobber: without this it may move them above it.  (Loads
+// through members of a parameter struct are ordinary ones, and need it for __ldg only.)
 template <typename... Pointer>
 __device__ __forceinline__ void fresh(Pointer&... p) {
   const int in_turn[] = {([](auto& q) { asm volatile("" : "+l"(q)); }(p), 0)...};

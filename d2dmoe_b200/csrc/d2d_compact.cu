@@ -70,6 +70,7 @@ compact_scatter_kernel(const uint32_t* __restrict__ mask_bits, const uint8_t* __
   for (int e = tid; e < 2 * EP; e += NTS) tot[e] = 0;      // tot and pre are adjacent
   __syncthreads();
   grid_dependency_wait();      // mask and counts table come from the previous kernel
+  fresh(mask_bits, counts);
   // this thread's mask words (one row of 32 tokens per warp); the loads are in flight during
   // the table sweep and the words stay in registers for both passes
   uint32_t word[MAX_E / 32];

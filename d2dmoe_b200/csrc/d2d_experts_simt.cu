@@ -70,7 +70,8 @@ experts_simt_kernel(const T* __restrict__ x, const int32_t* __restrict__ token_i
   const int row0 = 16 * rg + lr, col0 = CW * cg + 4 * lc;
   grid_launch_dependents();
   grid_dependency_wait();      // token lists and offsets come from the previous kernel
-  if (PAIRS) fresh(x, token_idx, offsets, w1, b1, w_up, w2);
+  fresh(x, token_idx, offsets);
+  if (PAIRS) fresh(w1, b1, w_up, w2);
 
   if (tid == 0) {
     int run = 0;

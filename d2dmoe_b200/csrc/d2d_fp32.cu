@@ -258,6 +258,7 @@ router_fp32_kernel(const float* __restrict__ x, const float* __restrict__ wa,
   const int64_t t0 = (int64_t)(blockIdx.x / CLUSTER) * TR;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(x);
   for (int i = tid; i < TR * EP; i += NT) share[i] = 0.f;
   const int slices = (R + TH - 1) / TH, chunks = (d + KC - 1) / KC;
   const int lr = lane >> 2, kl = w * KW + 4 * (lane & 3), dst = at_k(lr, lane & 3);
@@ -428,7 +429,8 @@ experts_fp32_kernel(const float* __restrict__ x, const int32_t* __restrict__ tok
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
-  if (PAIRS) fresh(x, token_idx, offsets, w1, b1, w2);
+  fresh(x, token_idx, offsets);
+  if (PAIRS) fresh(w1, b1, w2);
   for (int e = tid; e <= E; e += NT) off[e] = offsets[e];
   __syncthreads();
   if (w == 0) {                        // lane has experts 8 lane .. + 7

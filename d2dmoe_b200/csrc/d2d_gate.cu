@@ -70,6 +70,7 @@ router_mask_simt_kernel(const T* __restrict__ x, const T* __restrict__ wa,
   const int64_t t0 = (int64_t)blockIdx.x * TM_;
   grid_launch_dependents();
   grid_dependency_wait();      // x may come from the previous kernel of the stream
+  fresh(x);
   // vector staging needs rows that start on a 4-element boundary
   const bool vec = (d % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(wa)) % 16 == 0);
 
@@ -370,6 +371,7 @@ gate_scores_fused_kernel(const T* __restrict__ scores, float mult,
   for (int e = tid; e < E; e += NT) cnt[e] = 0;
   if (tid < 4) rows[tid] = 0u;
   grid_dependency_wait();
+  fresh(scores, x);
   // all rows: first, their stores depend on nothing the rule computes and drain while it runs
   if (out && !direct)
     init_tile_rows(x, last_bias, add_residual, out, t0, ntok, d, nullptr, w, lane);
@@ -455,6 +457,7 @@ gate_scores_fused_rows_kernel(const T* __restrict__ scores, float mult, int k, f
   const int ntok = (int)min((int64_t)128, N - t0);
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(scores, x);
   if (OTHERS) {
     if ((int)blockIdx.x >= ctas) {
       const int64_t n = (int64_t)gridDim.x - ctas, h = (int64_t)blockIdx.x - ctas, r0 = N * h / n;
@@ -558,6 +561,7 @@ all_experts_kernel(uint32_t* __restrict__ mask_bits, T* __restrict__ rt,
   const int nw = (E + 31) / 32;
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(x);
   const uint32_t n = (uint32_t)N, pairs = n * (uint32_t)E;         // < 2^31
   for (uint32_t i = (uint32_t)i0; i < pairs; i += (uint32_t)step) {
     token_idx[i] = (int32_t)(i % n);

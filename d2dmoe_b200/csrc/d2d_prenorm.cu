@@ -42,6 +42,7 @@ prenorm_init_kernel(const T* __restrict__ x, const T* __restrict__ gamma,
   constexpr int V = 16 / sizeof(T);
   grid_launch_dependents();
   grid_dependency_wait();
+  fresh(x);
   const int lane = threadIdx.x & 31;
   const int dv = d / V;                       // vectors per row
   const int nv = (dv + 31) / 32;              // vectors per lane (<= MAXV_)

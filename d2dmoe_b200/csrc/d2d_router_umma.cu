@@ -522,7 +522,7 @@ __device__ void role_init(const Params& p, Ctl* c, int w, int lane) {
           rr[u] = m != 0u && run ? __ffs(m) - 1 : -1;
           m &= m - 1;
           if (rr[u] >= 0)
-            xv[u] = __ldg(reinterpret_cast<const uint4*>(p.resid + (row0 + rr[u]) * p.d) + c8);
+            xv[u] = *(reinterpret_cast<const uint4*>(p.resid + (row0 + rr[u]) * p.d) + c8);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
@@ -567,7 +567,7 @@ __device__ __forceinline__ void help_init_rows(const Params& p) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)          // four rows in flight
         if (t + u * (NTHREADS / 32) < row1)
-          v[u] = __ldg(reinterpret_cast<const uint4*>(p.resid + (t + u * (NTHREADS / 32)) * p.d) + c8);
+          v[u] = *(reinterpret_cast<const uint4*>(p.resid + (t + u * (NTHREADS / 32)) * p.d) + c8);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (t + u * (NTHREADS / 32) < row1)
@@ -872,7 +872,7 @@ router_cluster_kernel(const Params p, const __grid_constant__ CUtensorMap tmx) {
         uint4 o = make_uint4(0u, 0u, 0u, 0u);
         if (p.last_bias) o = __ldg(reinterpret_cast<const uint4*>(p.last_bias) + c8);
         if (p.resid)
-          o = add_bf16x8(o, __ldg(reinterpret_cast<const uint4*>(p.resid + t * p.d) + c8));
+          o = add_bf16x8(o, *(reinterpret_cast<const uint4*>(p.resid + t * p.d) + c8));
         *(reinterpret_cast<uint4*>(p.out_init + t * p.d) + c8) = o;
       }
     }

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_operators import ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, within
+from test_operators import (ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, weighted_layer,
+                            within)
 
 
 # -- rows of pairs ------------------------------------------------------------------------------
@@ -131,3 +132,47 @@ def test_sum_of_rows_wider_than_a_quotients_range(dtype, d):
         want = float(w[t, 0]) * (h @ w2[i].double()) + lb.double()
         size = float(w[t, 0]) * (h_abs @ w2[i].double().abs()) + lb.double().abs()
         within(got[t], want, half(DT[dtype]) * want.abs() + (2 * 64 + H + 16) * U * size, t)
+
+
+# -- layers behind a kernel that lets them start early -----------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["all", "topk", "dynk", "dynk_max", "weighted"])
+@pytest.mark.parametrize("dtype,d", [("bf16", 256), ("fp32", 256), ("bf16", 100)])
+def test_layers_read_the_norm_of_this_replay(mode, dtype, d):
+    """The layer's kernels may start while layer_norm still writes x; replays on new inputs must see the new rows."""
+    import d2dmoe_b200 as D
+    torch.manual_seed(3)
+    norm = torch.nn.LayerNorm(d).to(DT[dtype]).cuda()
+    for N in (7, 300, 3000):
+        moe = weighted_layer(dtype, d=d, residual=True)
+        moe.forward_mode, moe.tau, moe.k = mode, 0.5, 4
+        h = randn(gen(N), 1, N, d).to(DT[dtype])
+
+        def step():
+            x = D.layer_norm(h, norm.weight.detach(), norm.bias.detach(), norm.eps)
+            y, gating = moe(x)
+            z, _ = moe.forward_block(x, norm)
+            return x, y, gating["ffn"][0], z
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s), torch.no_grad():
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr), torch.no_grad():
+            x, y, rt, z = step()
+        for turn in range(4):
+            h.copy_(randn(gen(100 * turn + N), 1, N, d) * (1 + turn))
+            gr.replay()
+            torch.cuda.synchronize()
+            with torch.no_grad():
+                xs = D.layer_norm(h, norm.weight.detach(), norm.bias.detach(), norm.eps)
+                torch.cuda.synchronize()
+                ys, gating = moe(xs)
+                torch.cuda.synchronize()
+                zs, _ = moe.forward_block(xs, norm)
+                torch.cuda.synchronize()
+            assert torch.equal(x, xs) and torch.equal(rt, gating["ffn"][0])
+            # (the 0/1 path adds in any order: about 2^-9 a sum; rows of another input differ by their own size)
+            for a, c in ((y, ys), (z, zs)):
+                assert ((a - c).float().norm(dim=-1) <= 0.1 * c.float().norm(dim=-1)).all()
