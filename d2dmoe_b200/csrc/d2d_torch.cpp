@@ -532,7 +532,8 @@ PyObject* run_host(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // One call from Python per operator: arguments are checked, outputs and workspaces allocated on the current stream, the C
 // ABI entered.  Each returns its outputs, or the status code (int) of a refused call.
 
-// a tensor argument, which must be on the GPU (and on that of `like`); None: null
+// a tensor argument, which must be on the GPU (and on that of `like`) and without a forward-mode tangent, which the result
+// would lose; None: null
 const at::Tensor* given(PyObject* o, const char* name, const at::Tensor* like = nullptr) {
   if (o == Py_None) return nullptr;
   const at::Tensor* t = tensor_of(o);
@@ -540,6 +541,8 @@ const at::Tensor* given(PyObject* o, const char* name, const at::Tensor* like = 
   TORCH_CHECK(t->is_cuda(), "d2dmoe_b200 runs on CUDA tensors only (there is no CPU path)");
   TORCH_CHECK_VALUE(!like || t->device() == like->device(), "tensors of one call live on different devices: ",
                     like->device(), " and ", t->device(), " (", name, ")");
+  TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), "d2dmoe_b200's operators have no forward-mode derivative (",
+                              name, " has a tangent)");
   return t;
 }
 

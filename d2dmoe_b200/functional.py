@@ -1,7 +1,8 @@
 """Differentiable operators in front of the layer: its norm, and routing with weights.
 
 Both run under autograd over the CUDA library (``ops.layer_norm`` / ``ops.route`` and their backward
-passes, in native code); without a gradient to compute they are the plain calls.  First derivatives only.
+passes, in native code); without a gradient to compute they are the plain calls.  First derivatives in reverse mode only:
+a tensor with a forward-mode tangent is refused.
 """
 from __future__ import annotations
 

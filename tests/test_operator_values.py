@@ -114,6 +114,33 @@ def test_a_nan_stays_one_through_the_unweighted_layer(dtype, d, H, N):
     assert torch.isfinite(out).all()
 
 
+# -- forward mode -------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    """No operator has a forward-mode derivative; a result without its tangent would be wrong without a word."""
+    import torch.autograd.forward_ad as fw
+    import d2dmoe_b200 as D
+    g = gen(9)
+    x, w, b = randn(g, 20, 48), 1 + randn(g, 48), randn(g, 48)
+    ex = weighted_layer(d=256).experts
+    h = randn(g, 20, 256).bfloat16()
+    wt, e = D.route_tokens(randn(g, 20, 24), 4)
+    y, mean, rstd = D.ops.layer_norm(x, w, b)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        calls = [lambda: D.layer_norm(dual(x), w, b), lambda: D.layer_norm(x, dual(w), b),
+                 lambda: D.layer_norm(x, w, dual(b)), lambda: D.layer_norm(dual(x.requires_grad_()), w, b),
+                 lambda: D.ops.layer_norm_backward(dual(y), x.detach(), w, mean, rstd),
+                 lambda: D.route_tokens(dual(x), 3), lambda: D.route_tokens(x, 3, bias=dual(b)),
+                 lambda: ex.forward_weighted(dual(h), e, wt), lambda: ex.forward_weighted(h, e, dual(wt))]
+        for n, call in enumerate(calls):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {n} dropped its tangent")
+    ex.forward_weighted(h, e, wt)
+
+
 # -- rows wider than 2^16 -----------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [("fp32", 70001), ("bf16", 100003)])
