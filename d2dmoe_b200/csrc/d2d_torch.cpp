@@ -1044,7 +1044,10 @@ PyObject* run_weighted(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int residual = PyObject_IsTrue(a[8]);
   const at::Tensor* status = given(a[9], "status", &xt);
   if (PyErr_Occurred()) return nullptr;
-  use_on(*p, c10::cuda::getCurrentCUDAStream(p->device.index()));
+  const auto cur = c10::cuda::getCurrentCUDAStream(p->device.index());
+  use_on(*p, cur);
+  // (the word is the module's: it may be gone before this call has run)
+  if (status) c10::cuda::CUDACachingAllocator::recordStream(status->storage().data_ptr(), cur);
   const ExpertWeights m = {p->w1, p->b1, p->wup, p->w2, p->ep, p->E, p->d, p->H, (int)p->act, p->dtype};
   return run_weighted_experts(m, xt, et, wt, bias, residual, status);
   END_HANDLE_TH_ERRORS

@@ -169,7 +169,10 @@ class _StatusWords(dict):
 
     def __missing__(self, device):
         _not_in_a_capture()
-        w = self[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        w = torch.zeros(1, dtype=torch.int32, device=device)
+        # calls on any stream may report from now on: not before the zero is there
+        torch.cuda.current_stream(device).synchronize()
+        self[device] = w
         return w
 
     def __deepcopy__(self, memo):
@@ -299,6 +302,8 @@ class B200KernelExperts(ExpertsLayer):
             self._image_before_capture()
         with torch.no_grad():
             p = self.kernel_params()
+            if status is not None:
+                status.record_stream(torch.cuda.current_stream(x.device))
             return ops.experts_weighted(x, experts, weights, p["w1"], p["b1"], p["w2"], p["act"], w_up=p["w_up"],
                                         packed=self.packed(), last_bias=last_bias, add_residual=add_residual,
                                         status=status)
@@ -346,11 +351,14 @@ class B200KernelExperts(ExpertsLayer):
         return words
 
     def check_status(self):
-        """Raise D2DError for what a kernel of an earlier ``forward_weighted`` reported (synchronises)."""
-        for w in self._status_words().values():
+        """Raise D2DError for what a kernel of an earlier ``forward_weighted`` reported, on whatever stream (waits for
+        all streams of the devices that such calls ran on)."""
+        for device, w in self._status_words().items():
+            torch.cuda.synchronize(device)
             code = int(w.item())
             if code:
                 w.zero_()
+                torch.cuda.current_stream(device).synchronize()
                 raise D2DError(code, "device status")
 
     # -- router-training labels as a by-product of the expert kernel ----------------------

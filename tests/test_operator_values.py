@@ -141,6 +141,38 @@ def test_tangents_are_refused():
     ex.forward_weighted(h, e, wt)
 
 
+# -- the status word across streams ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [False, True])
+def test_status_of_calls_on_other_streams(first):
+    """check_status knows what calls on any stream reported, and the word's first value is there before all of them."""
+    from d2dmoe_b200._capi import D2DError
+    ex = weighted_layer().experts
+    ex.packed()
+    torch.cuda.synchronize()
+    x, w = randn(gen(1), 6, 256).bfloat16(), torch.ones(6, 4, device="cuda")
+    good = torch.zeros(6, 4, dtype=torch.int32, device="cuda")
+    wrong = torch.full_like(good, 99)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    if first:                                            # the word is made on a stream that is busy
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(100_000_000)
+            ex.forward_weighted(x, good, w)
+        with torch.cuda.stream(b):
+            ex.forward_weighted(x, wrong, w)
+        torch.cuda.synchronize()
+    else:
+        ex.forward_weighted(x, good, w)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(100_000_000)
+            ex.forward_weighted(x, wrong, w)
+    with pytest.raises(D2DError):
+        ex.check_status()
+    ex.check_status()
+
+
 # -- rows wider than 2^16 -----------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [("fp32", 70001), ("bf16", 100003)])
