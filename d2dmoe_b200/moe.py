@@ -567,8 +567,9 @@ class MoeficationMoE(MoELayer):
     ``forward(x[B,S,d]) -> (out[B,S,d], {name: (routing_tensor[B,S,E],)})`` with
     ``forward_mode`` in {'all','topk','dynk','dynk_max'}, ``tau``/``k`` read at call
     time; and 'weighted', which upstream has not: the router's output as logits of ``routing``
-    (a ``Routing``), ``k`` experts per token, their outputs weighted and summed; its routing tensor holds the weights.  In every mode the whole layer is one native call (router + rule -> bit mask ->
-    token lists -> expert FFN with scatter-add); a router that is not the D2DMoE form runs as
+    (a ``Routing``), ``k`` experts per token, their outputs weighted and summed; its routing tensor holds the weights (a token
+    with a NaN or +inf logit: NaN in the output, zeros there).  In the other modes the whole layer is one native call
+    (router + rule -> bit mask -> token lists -> expert FFN with scatter-add); a router that is not the D2DMoE form runs as
     the module it is and hands over its scores.
     ``tau`` keeps the upstream meaning: expert e runs iff score_e >= max_e(score)*(1.0-tau).
     """
@@ -636,6 +637,9 @@ class MoeficationMoE(MoELayer):
     @torch.no_grad()
     def _forward_weighted(self, x):
         weights, experts, rt = self._route(x)
+        # A token with a NaN or +inf logit has NaN weights and no experts.  Its sum is NaN, as the weights say, not that of
+        # a token without experts: any expert will do to carry them there.
+        experts.masked_fill_(weights.isnan(), 0)
         out = self.experts.forward_weighted(x, experts, weights,
                                             last_bias=self.last_bias.view(-1) if self.bias else None,
                                             add_residual=self.add_residual_connection)

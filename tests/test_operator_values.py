@@ -114,6 +114,38 @@ def test_a_nan_stays_one_through_the_unweighted_layer(dtype, d, H, N):
     assert torch.isfinite(out).all()
 
 
+# -- a token whose logits are NaN, in the layer -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,glu", [("bf16", False), ("bf16", True), ("fp32", False)])
+@pytest.mark.parametrize("N", [3, 900])
+def test_a_token_without_usable_logits_shows_in_the_layers_output(N, dtype, glu):
+    """Its weights are NaN, and so is its row; a token that no expert is allowed for has the bias."""
+    moe = weighted_layer(dtype, glu)
+    bad = torch.zeros(24, device="cuda", dtype=DT[dtype])
+
+    class Router(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            s = self.inner(x)
+            s[0, 1, 3], s[0, 2, 4] = math.nan, math.inf
+            s[0, 0] = -math.inf
+            return s + bad
+    x = randn(gen(2), 1, N, 256).to(DT[dtype])
+    with torch.no_grad():
+        moe.router = Router(moe.router)
+        out, gating = moe(x)
+        lb = moe.last_bias.view(-1) if moe.bias else torch.zeros(256, device="cuda", dtype=DT[dtype])
+        assert torch.isnan(out[0, 1:3]).all() and torch.equal(out[0, 0], lb)
+        assert torch.isfinite(out[0, 3:]).all() and not gating["ffn"][0][0, :3].any()
+        other = x.clone()
+        other[0, :3] = 0.5
+        assert torch.equal(moe(other)[0][0, 3:], out[0, 3:])
+    moe.experts.check_status()
+
+
 # -- forward mode -------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_tangents_are_refused():
