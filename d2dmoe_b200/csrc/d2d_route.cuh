@@ -492,12 +492,16 @@ __global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ?
             at = at + 1 == n ? 0 : at + 1;
           }
           value[g] = second > -INFINITY ? best + second : best;
+          // How far that can be off: the bound of single scores, below, for both and their sum.  It goes by their size, which
+          // cancels in the sum.  (No expert left: nothing to be off; a sum that is not finite is not known at all.)
+          const float most = fmaxf(fabsf(best), second > -INFINITY ? fabsf(second) : 0.f);
+          value[a.groups + g] = best > -INFINITY ? fmaf(most, 5e-7f, 6e-6f) : 0.f;
         }
         __syncwarp();
         uint32_t kept = 0u;
-        float worst = INFINITY, other = -INFINITY;       // kept, not kept
+        float worst = INFINITY, other = -INFINITY;       // the least a kept group can be, the most another one
         for (int g = q; g < a.groups; g += L) {
-          const float v = value[g];
+          const float v = value[g], off = value[a.groups + g];
           int before = 0;
 #pragma unroll 4
           for (int h = 0; h < a.groups; ++h) {
@@ -506,9 +510,9 @@ __global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ?
           }
           if (before < a.top_groups) {
             kept |= 1u << g;
-            worst = fminf(worst, v);
-          } else {
-            other = fmaxf(other, v);
+            worst = fminf(worst, v - off);
+          } else if (off > 0.f) {
+            other = fmaxf(other, fmaxf(v + off, -MAX_FINITE));
           }
         }
 #pragma unroll
@@ -517,8 +521,7 @@ __global__ void __launch_bounds__(NT, KP == 16 ? 4 : MODE == ORDER ? (EL == 32 ?
           worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
           other = fmaxf(other, __shfl_xor_sync(0xffffffffu, other, o));
         }
-        // (two scores and their sum: twice the bound of single ones, below)
-        unsure = other > -INFINITY && worst - other <= 1.2e-5f + 1e-6f * fabsf(worst);
+        unsure = other > -INFINITY && !(worst > other);
 #pragma unroll
         for (int v = 0; v < EL / V; ++v) {
           const int e = (v * L + q) * V;

@@ -146,6 +146,28 @@ def test_a_token_without_usable_logits_shows_in_the_layers_output(N, dtype, glu)
     moe.experts.check_status()
 
 
+# -- groups whose two best cancel --------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_groups_whose_scores_and_biases_cancel(scores, dtype):
+    """A group counts as the sum of its two best score + bias, whose size says nothing about their roundings."""
+    g = gen(21)
+    logits = randn(g, 300, 16).to(DT[dtype])
+    for big in (3.0, 1000.0, 30000.0):
+        # (the larger c of the groups lie apart and within 4 of each other: only the groups are in question)
+        bias = torch.empty(16, device="cuda")
+        bias[0::2] = big + 0.4 * torch.randperm(8, generator=g, device="cuda")
+        bias[1::2] = -bias[0::2]
+        check_route(logits, 3, bias=bias, groups=8, top_groups=3, scores=scores)
+        bias[5] = bias[8] = -1e9                         # groups far behind
+        check_route(logits, 3, bias=bias, groups=8, top_groups=3, scores=scores)
+    # sums that 32 bits do not hold, and cannot order
+    for sign in (1.0, -1.0):
+        bias = sign * 2e38 * (1 + 0.05 * torch.randperm(8, generator=g, device="cuda").float()).repeat_interleave(2)
+        check_route(logits, 4, bias=bias, groups=8, top_groups=3, scores=scores)
+
+
 # -- forward mode -------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_tangents_are_refused():
