@@ -148,12 +148,15 @@ int d2d_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
                               dtype, param_dtype, ws, (cudaStream_t)stream);
 }
 
+// positive, normal (the gradient divides by it) and finite
+static bool scale_ok(float scale) { return scale >= 1.175494351e-38f && scale <= 3.402823466e38f; }
+
 int d2d_route(const void* logits, const float* bias_opt, int scores, int k, int groups, int top_groups,
               int renormalise, float scale, int32_t* experts, float* weights, uint32_t* mask_bits_opt,
               void* routing_tensor_opt, int64_t N, int E, int dtype, d2d_stream_t stream) {
   if (!logits || !experts || !weights || N < 0 || E < 1 || k < 1 || k > E || groups < 1 || E % groups != 0 ||
       top_groups < 1 || top_groups > groups || k > E / groups * top_groups ||
-      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
+      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !scale_ok(scale))
     return D2D_ERR_BAD_ARG;
   if (!dtype_ok(dtype) || E > ROUTE_MAX_E || k > ROUTE_MAX_K || groups > ROUTE_MAX_GROUPS)
     return D2D_ERR_UNSUPPORTED;
@@ -170,7 +173,7 @@ int d2d_route_backward(const void* logits, const int32_t* experts, const float* 
                        int scores, int renormalise, float scale, void* dlogits, int64_t N, int E, int k, int dtype,
                        d2d_stream_t stream) {
   if (!logits || !experts || !weights || !dweights || !dlogits || N < 0 || E < 1 || k < 1 || k > E ||
-      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !(scale > 0.f) || scale > 3.402823466e38f)
+      (scores != D2D_SCORES_SOFTMAX && scores != D2D_SCORES_SIGMOID) || !scale_ok(scale))
     return D2D_ERR_BAD_ARG;
   if (!dtype_ok(dtype) || E > ROUTE_MAX_E || k > ROUTE_MAX_K) return D2D_ERR_UNSUPPORTED;
   if (N == 0) return D2D_OK;

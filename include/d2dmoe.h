@@ -253,7 +253,7 @@ int d2d_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, in
  * out of the choice; slots for which none is left have expert -1 and weight 0.  A token with a NaN or +inf among its
  * logits or biases has experts -1 and weights NaN.  Optional outputs: mask_bits (what d2d_compact reads) and the
  * routing tensor [N, E] in T with the weights in place of ones.
- * 1 <= k <= min(32, E / groups * top_groups), E <= 1024, groups <= 32 divides E, scale > 0.
+ * 1 <= k <= min(32, E / groups * top_groups), E <= 1024, groups <= 32 divides E, scale a positive normal number.
  * (Upstream's 'topk' gate, architectures/moe/moefication.py:59-63, keeps 0/1 decisions of raw scores.) */
 #define D2D_SCORES_SOFTMAX 0
 #define D2D_SCORES_SIGMOID 1

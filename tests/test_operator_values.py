@@ -289,3 +289,22 @@ def test_layers_read_the_norm_of_this_replay(mode, dtype, d):
             # (the 0/1 path adds in any order: about 2^-9 a sum; rows of another input differ by their own size)
             for a, c in ((y, ys), (z, zs)):
                 assert ((a - c).float().norm(dim=-1) <= 0.1 * c.float().norm(dim=-1)).all()
+
+
+# -- scales -------------------------------------------------------------------------------------------------------
+def test_scales_without_a_reciprocal_are_refused():
+    """The gradient divides the weights by their scale: one below the normal numbers has no finite reciprocal."""
+    import ctypes as C
+    from d2dmoe_b200 import _capi
+    a = C.c_void_p(0x7f0000000000)
+    for scale, want in ((1e-39, 1), (2.0 ** -149, 1), (2.0 ** -126, 0), (3e38, 0)):
+        assert _capi.lib.d2d_route(a, None, 0, 4, 1, 1, 1, scale, a, a, None, None, 0, 24, 1, None) == want
+        assert _capi.lib.d2d_route_backward(a, a, a, a, 0, 1, scale, a, 0, 24, 4, 1, None) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 100])
+def test_gradient_at_extreme_scales(scale):
+    g = gen(6)
+    for how in (dict(), dict(scores="sigmoid"), dict(renormalise=False)):
+        check_route(randn(g, 40, 24), 4, randn(g, 40, 4), scale=scale, **how)
