@@ -172,8 +172,7 @@ class _StatusWords(dict):
         w = torch.zeros(1, dtype=torch.int32, device=device)
         # calls on any stream may report from now on: not before the zero is there
         torch.cuda.current_stream(device).synchronize()
-        self[device] = w
-        return w
+        return self.setdefault(device, w)            # (another thread's first call may have come in between)
 
     def __deepcopy__(self, memo):
         return _StatusWords()

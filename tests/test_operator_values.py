@@ -227,6 +227,34 @@ def test_status_of_calls_on_other_streams(first):
     ex.check_status()
 
 
+@pytest.mark.gpu
+def test_status_of_first_calls_from_several_threads():
+    """They share one word, whichever of them makes it."""
+    import threading
+    from d2dmoe_b200._capi import D2DError
+    x, w = randn(gen(1), 6, 256).bfloat16(), torch.ones(6, 4, device="cuda")
+    good = torch.zeros(6, 4, dtype=torch.int32, device="cuda")
+    wrong = torch.full_like(good, 99)
+    for turn in range(8):
+        ex = weighted_layer().experts
+        ex.packed()
+        torch.cuda.synchronize()
+        start = threading.Barrier(8)
+
+        def call(i):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                torch.cuda._sleep(1_000_000 * (i + 1))
+                start.wait()
+                ex.forward_weighted(x, wrong if i == turn else good, w)
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        with pytest.raises(D2DError):
+            ex.check_status()
+
+
 # -- rows wider than 2^16 -----------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [("fp32", 70001), ("bf16", 100003)])
