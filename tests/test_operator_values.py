@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from test_operators import (ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, weighted_layer,
-                            within)
+from test_operators import (ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, route_gradient,
+                            route_reference, weighted_layer, within)
 
 
 # -- rows of pairs ------------------------------------------------------------------------------
@@ -336,3 +336,33 @@ def test_gradient_at_extreme_scales(scale):
     g = gen(6)
     for how in (dict(), dict(scores="sigmoid"), dict(renormalise=False)):
         check_route(randn(g, 40, 24), 4, randn(g, 40, 4), scale=scale, **how)
+
+
+# -- offsets past 32 bits -------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_routing_gradient_past_32_bits():
+    """Rows of dlogits on either side of 2^31 elements and at the end, against the 64-bit gradient."""
+    import d2dmoe_b200 as D
+    g = gen(1)
+    N, E, k = 17_000_000, 128, 2
+    logits = torch.empty(N, E, dtype=torch.bfloat16, device="cuda")
+    for part in logits.split(1 << 20):
+        part.copy_(randn(g, *part.shape))
+    dw = randn(g, N, k)
+    rows = torch.tensor([0, 16_777_215, 16_777_216, N - 1], device="cuda")
+    few = logits[rows].double().cpu()
+    rel = (96 + 4 * (few.amax(1) - few.amin(1))[:, None]) * U
+    for how in (dict(), dict(scores="sigmoid"), dict(renormalise=False)):
+        how = dict(dict(scores="softmax", renormalise=True, scale=1.0), **how)
+        w, e, _ = D.ops.route(logits, k, **how)
+        got = D.ops.route_backward(dw, logits, e, w, **how)[rows].cpu()
+        W, I, S = route_reference(logits[rows], k, **how)
+        assert torch.equal(e[rows].cpu(), I)
+        want = route_gradient(logits[rows], dw[rows], I, **how)
+        gd = dw[rows].double().cpu().abs()
+        dot = (W * gd).sum(1, keepdim=True)              # what cancels, per row
+        size = torch.zeros_like(want).scatter_add_(1, I.long(), W * (gd + dot))
+        if how["scores"] == "softmax" and not how["renormalise"]:
+            size = S * dot + size
+        within(got, want, half(logits.dtype) * want.abs() + 4 * rel * size + 1e-37, how)
+        del w, e, got
