@@ -16,9 +16,10 @@
 //   * a thread has the same columns of every row its block takes, so the column sums of the backward pass are running sums in
 //     its registers; a block writes one partial row of them at its end, and a second kernel adds the partial rows in the
 //     order of the blocks.  No atomics: the same call gives the same bits.
-// Of the measured copy rate (6.5 TB/s): forward 87 % at 50432 x 768, 82 % at 32768 x 2048; backward 75 % there, 84 % at
-// 40000 x 1024 fp32, 63 % at 50432 x 768 (56 us, 43 without the column sums: 24 columns a lane and their two sums take all 128
-// registers, and the second kernel some 4 us).
+// Of the measured copy rate (6.5 TB/s), calls one after another, the second kernel within them: forward 88 % at 50432 x 768
+// (27 us), 83 % at 32768 x 2048 (50), 81 % at 40000 x 1024 fp32 (62); backward 74 % (83 us), 83 % (90) and, at 50432 x 768, 63 %
+// (56 us, 43 without the column sums: 24 columns a lane and their two sums take all 128 registers, and the second kernel some 4 us).
+// Rows that no vector divides go one element a load: 4099 x 1023 fp32 forward 36 %, backward 39 % (14 and 20 us).
 // Statistics, both row sums and all column sums are held in 32 bits; each output is rounded once.
 #include <algorithm>
 

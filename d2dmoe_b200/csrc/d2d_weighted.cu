@@ -10,7 +10,8 @@
 //           310 MB each way next to 155 MB of x and out).  The tensor-core kernel's rows are 16 bits an
 //           element, in a format of its own (encode8) that is off by 2^-14 of the largest of eight where bf16 would be by 2^-8 of each
 //           (error of a gated call against 64 bits 2.4e-3 instead of 2.8e-3 of the 2-norm, 1.7e-3 of it the result's own
-//           rounding); the fp32 and the general-shape kernel's are fp32.  50432 x 768, 4 of 24 experts: sort 11, experts 112, sum 78 us.
+//           rounding); the fp32 and the general-shape kernel's are fp32.  50432 x 768, 4 of 24 experts: sort 11, experts 112, sum 78 us,
+//           each by itself; the call 223.
 //   few     Calls of few pairs are bound by latency and by the weights' bytes: two kernels without lists, all
 //           sums in 32 bits.  Blocks share out a pair's hidden columns in the first, a token's columns in the second;
 //           where those are fewer than the SMs take, clusters split the depth, or the slots, and meet in distributed
@@ -636,8 +637,11 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // tokens x 8 34 / 58, 37 tokens 59 / 60, 48 tokens 84 / 61; 768 x 128, 24 experts (393 KB) 48 tokens x 4 14 / 17, 64 tokens
 // 16.5 / 16.6, 96 tokens 20 / 16.5; 768 x 32 (98 KB) 197 tokens x 4 15 / 21.  fp32, whose lists take the longer the larger an expert
 // is: 768 x 128 (786 KB) 96 tokens x 4 31 / 35, 128 tokens 40 / 33; 768 x 32 (197 KB) 197 tokens x 4 25 / 29, 256 tokens 31 / 29;
-// 1024 x 512 (4.2 MB) 64 tokens x 2 53 / 75, 128 tokens 96 / 73.  Where lists mean the general-shape kernel, measured on
-// fp32 768 x 128: 256 tokens x 4 74 / 128, 400 tokens 111 / 119.
+// 1024 x 512 (4.2 MB) 64 tokens x 2 53 / 75, 128 tokens 96 / 73.  Where lists mean the general-shape kernel the line is that of
+// fp32 768 x 128 (256 tokens x 4 74 / 128, 400 tokens 111 / 119), for shapes whose own lines lie on either side of it: bf16
+// 130 x 20 682 tokens x 3 25 / 32; bf16 1000 x 100, whose 100 no 16-byte vector divides, 128 tokens x 4 100 / 123, 256 tokens 188 / 168,
+// 512 tokens 366 / 171; 1001 x 100 256 tokens 188 / 285, 512 tokens 366 / 304; gated 768 x 128 fp32 256 tokens x 4 96 / 188, 512
+// tokens 182 / 204, bf16 without packed weights 512 tokens 117 / 225; gated 2048 x 128 fp32 64 tokens x 8 192 / 554.
 bool takes_few(int64_t P, int d, int E, int H, int k, bool glu, int dtype, bool tiles) {
   const int64_t expert = (int64_t)(glu ? 3 : 2) * d * H * (dtype == D2D_F32 ? 4 : 2);
   const bool fp32 = dtype == D2D_F32 && !glu && experts_fp32_pairs_supported(d, E, H);
