@@ -578,8 +578,9 @@ int backward_t(const T* dy, const T* x, const P* gamma, const float* mean, const
     const int vpt = ceil_div(nv, s.tpr);
     return vpt <= 1   ? backward_vpt<T, P, VW, 1>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)
            : vpt <= 2 ? backward_vpt<T, P, VW, 2>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)
-           : vpt <= 3 ? backward_vpt<T, P, VW, 3>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)
-                      : backward_vpt<T, P, VW, 4>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st);
+           : vpt <= 3 && (VW == 4 || s.tpr <= BLOCK)         // (512 threads, bf16: its ring and parameters are 246 KB)
+               ? backward_vpt<T, P, VW, 3>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st)
+               : backward_vpt<T, P, VW, 4>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part, s, sms, st);
   }
   nv = s.d;
   s.tpr = threads_per_row(nv, nv <= 128 ? 4 : 8);

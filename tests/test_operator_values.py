@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from test_operators import (ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, randn, route_gradient,
-                            route_reference, weighted_layer, within)
+from test_operators import (ACTS, DT, U, check_route, experts_case, experts_reference, gen, half, norm_inputs,
+                            norm_reference, randn, route_gradient, route_reference, weighted_layer, within)
 
 
 # -- rows of pairs ------------------------------------------------------------------------------
@@ -366,3 +366,24 @@ def test_routing_gradient_past_32_bits():
             size = S * dot + size
         within(got, want, half(logits.dtype) * want.abs() + 4 * rel * size + 1e-37, how)
         del w, e, got
+
+
+# -- norms of long rows --------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,params", [("bf16", "same"), ("bf16", "fp32"), ("fp32", "same")])
+def test_norms_of_rows_of_every_length(dtype, params):
+    """Each number of vectors a thread can have, whole and ragged, up to the longest rows."""
+    import d2dmoe_b200 as D
+    for d in (4096, 4104, 6144, 6152, 8192, 8196, 8200, 9000, 10240, 12288, 12296, 14336, 16380, 16384, 8193, 12001):
+        for kind in ("layer", "rms"):
+            x, w, b, dy = norm_inputs(3, d, dtype, params, kind, 0)
+            ref = norm_reference(x, w, b, 1e-5, kind, 0.0, dy)
+            y, mean, rstd = D.ops.layer_norm(x, w, b, kind=kind)
+            within(y, *ref["y"], d)
+            dx, dw, db = D.ops.layer_norm_backward(dy, x, w, mean, rstd, kind=kind, bias=b is not None)
+            within(dx, *ref["dx"], d)
+            within(dw, *ref["dw"], d)
+            if b is not None:
+                within(db, *ref["db"], d)
+            only, _, _ = D.ops.layer_norm_backward(dy, x, w, mean, rstd, kind=kind, bias=False, dweight=False)
+            assert torch.equal(only, dx)
