@@ -55,6 +55,10 @@ struct RouteArgs {
 __device__ __forceinline__ bool unusable(float v) { return !(v <= MAX_FINITE); }      // NaN, +inf
 
 __device__ __forceinline__ float sigmoidf(float l) { return 1.f / (1.f + expf(-l)); }
+// sigmoid(l) e^-m for m <= 0 and the largest l of those whose quotients are wanted, or 0: as large as they are, none underflows
+__device__ __forceinline__ float scaled_sigmoid(float l, float m) {
+  return (l < 0.f ? expf(l - m) : 1.f) / (1.f + expf(-fabsf(l)));
+}
 
 constexpr float LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float exp2_fast(float v) {
@@ -89,11 +93,10 @@ __device__ __forceinline__ void put_choice(const RouteArgs& a, int64_t t, int q,
   float sum = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    // (sigmoids below e^-60 are exponentials to the last bit: their quotients do not underflow as those)
-    w[r] = e[r] < 0          ? 0.f
-           : !a.renormalise  ? (a.softmax ? softmax_term(l[r], m) / denom : sigmoidf(l[r]))
-           : a.softmax || mx < -60.f ? expf(l[r] - mx)
-                                     : sigmoidf(l[r]);
+    w[r] = e[r] < 0         ? 0.f
+           : !a.renormalise ? (a.softmax ? softmax_term(l[r], m) / denom : sigmoidf(l[r]))
+           : a.softmax      ? expf(l[r] - mx)
+                            : scaled_sigmoid(l[r], fminf(mx, 0.f));
     sum += w[r];
   }
   if (a.renormalise) {

@@ -387,3 +387,16 @@ def test_norms_of_rows_of_every_length(dtype, params):
                 within(db, *ref["db"], d)
             only, _, _ = D.ops.layer_norm_backward(dy, x, w, mean, rstd, kind=kind, bias=False, dweight=False)
             assert torch.equal(only, dx)
+
+
+# -- shares of small sigmoids ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("k", [8, 17])
+def test_shares_of_sigmoids_that_underflow(k, dtype):
+    """sigmoid(-95) is no 32-bit number, its share beside sigmoid(-50) is."""
+    g = gen(k)
+    for top in (-55.0, -30.0, -1.0, 2.0):
+        logits = (top - 60 * torch.rand(100, 24, generator=g, device="cuda")).to(DT[dtype])
+        check_route(logits, k, randn(g, 100, k), scores="sigmoid")
+        check_route(logits, k, scores="sigmoid", bias=0.1 * randn(g, 24), scale=2.5)
