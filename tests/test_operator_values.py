@@ -42,7 +42,7 @@ def test_rows_of_pairs_keep_their_size(glu):
         within(got, want.expand_as(got), tol.expand_as(got), e)
         along += float(((got[0] - want) * y).sum())
         size += float((y * y).sum())
-    # 3072 errors of at most 2^-14 of about twice the value, either way: 2^-13 / sqrt(3 * 3072) = 1.3e-6 of the whole
+    # E d errors of at most 2^-14 of about twice the value, either way: 2^-13 / sqrt(3 E d) = 1.3e-6 of the whole
     assert abs(along / size) <= 1e-5
 
 
